@@ -16,49 +16,15 @@
 #include "qmla_aux.cuh"
 #include "qmla_dcp.cuh"
 #include "qmla_decode.cuh"
+#include "qmla_host.cuh"
 
 using namespace qmla;
 
 namespace {
 
-constexpr int kMaxDynSmem = 232448;  // 227 KB opt-in limit per block on sm_100
 constexpr int kMaxRing = 12;         // K / V ring slots at most (bounds the barrier area)
 
-struct DevInfo {
-  int sms = 0;
-  int max_smem = 0;
-  bool ok = false;
-};
-
 std::mutex g_mu;
-std::map<int, DevInfo> g_dev;
-
-DevInfo dev_info(int dev) {
-  std::lock_guard<std::mutex> lk(g_mu);
-  auto it = g_dev.find(dev);
-  if (it != g_dev.end()) return it->second;
-  DevInfo d;
-  if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
-      cudaDeviceGetAttribute(&d.max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) ==
-          cudaSuccess)
-    d.ok = true;
-  g_dev[dev] = d;
-  return d;
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
 
 using MapKey = std::tuple<const void*, int, int, int, int64_t, int64_t, int64_t, int, int>;
 std::map<MapKey, CacheMaps> g_maps;
@@ -132,43 +98,6 @@ int cache_tensor_map(const qmla_decode_params* p, int run, int vcols, CacheMaps*
   *out = m;
   return QMLA_OK;
 }
-
-int gcd_int(int a, int b) {
-  while (b) {
-    int t = a % b;
-    a = b;
-    b = t;
-  }
-  return a;
-}
-
-int64_t align_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
-
-// Makes `dev` the current device for the lifetime of the guard and puts the caller's current
-// device back on every return path, so an entry point never leaves a thread that drives several
-// GPUs pointed at another one.
-class DeviceGuard {
- public:
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev_) != cudaSuccess) return;
-    if (prev_ == dev) {
-      ok_ = true;
-      return;
-    }
-    ok_ = cudaSetDevice(dev) == cudaSuccess;
-    switched_ = ok_;
-  }
-  ~DeviceGuard() {
-    if (switched_) cudaSetDevice(prev_);
-  }
-  bool ok() const { return ok_; }
-  DeviceGuard(const DeviceGuard&) = delete;
-  DeviceGuard& operator=(const DeviceGuard&) = delete;
-
- private:
-  int prev_ = -1;
-  bool ok_ = false, switched_ = false;
-};
 
 struct Plan {
   int fold, R, work_rows;  // decode rows folded into one work row, its query rows, work rows
