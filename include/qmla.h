@@ -256,6 +256,72 @@ typedef struct qmla_gather_params {
 
 int qmla_gather_cache(const qmla_gather_params* p, void* stream);
 
+/* ---- rotary positions -----------------------------------------------------
+ * x [tokens][heads][head_dim] -> out, both with any token / head strides (elements; unit stride
+ * on the last dim).  Dims [start, start + blocks * rot_dim) of every head turn, rot_dim at a time
+ * (a window of `blocks` packed groups); the others are copied.  Pair i of a block is
+ * dims (2i, 2i + 1) when interleaved, else (i, i + rot_dim / 2), and turns by
+ * 2 pi * frac(position * steps[i] / 2^64): steps[rot_dim / 2] holds each pair's turns per position
+ * as a 64-bit binary fraction, so angles stay exact at every position, negative ones included.
+ * cos and sin are multiplied by `scale` (long-context scalings).  adjoint = 1 applies the
+ * transpose, which is the gradient's way back.  out may be x itself (same strides): then only
+ * the window is touched.  Arithmetic is 32-bit, rounded once to dtype. */
+typedef struct qmla_rotary_params {
+  const void* x;
+  int64_t x_stride_token, x_stride_head;
+  void* out;
+  int64_t out_stride_token, out_stride_head;
+  int64_t num_tokens;
+  int32_t num_heads, head_dim;
+  int32_t dtype; /* QMLA_DT_BF16, QMLA_DT_F16 or QMLA_DT_F32 */
+  int32_t start, rot_dim, blocks; /* rot_dim even, <= 512 */
+  int32_t interleaved, adjoint;
+  float scale;
+  const void* positions; /* [num_tokens] int32, or int64 when positions_i64 */
+  int32_t positions_i64;
+  const int64_t* steps; /* [rot_dim / 2] */
+  int32_t device;
+} qmla_rotary_params;
+
+int qmla_rotary(const qmla_rotary_params* p, void* stream);
+
+/* A step's new tokens in one launch: q_pe [tokens][heads][rope_width] (bf16) -> q_out rotated, and
+ * for each token the cache row slot_mapping[i] = page * page_size + offset is written as
+ *   [latent (rank) | rotated rope keys (rope_width) | rms tail]
+ * from latent [tokens][rank] and k_pe [tokens][rope_width + rms_heads] ([rope | rms]), both bf16.
+ * rope_width is a whole number of rot_dim blocks.  bf16 cache: rms_mode NATIVE (copied) or NONE.
+ * FP8 cache: x / k_scale rounded once to e4m3 (saturating), rms tail as qmla_fp8_cache_write's
+ * (LOG8 or BF16) or NONE.  A negative slot writes no row (padding; its q is rotated all the same).
+ * A slot past num_pages * page_size writes none either and ORs QMLA_STATUS_BAD_INDEX into *status
+ * (when status is not NULL).  q_out may be q_pe itself. */
+typedef struct qmla_rope_cache_params {
+  const void* q_pe;
+  int64_t q_stride_token, q_stride_head;
+  void* q_out;
+  int64_t q_out_stride_token, q_out_stride_head;
+  const void* latent;
+  int64_t latent_stride;
+  const void* k_pe;
+  int64_t k_pe_stride;
+  const void* positions; /* [num_tokens] int32, or int64 when positions_i64 */
+  const int64_t* slot_mapping;
+  const int64_t* steps;
+  void* kv_cache;
+  int64_t kv_stride_page, kv_stride_token; /* elements */
+  int64_t num_tokens;
+  int32_t num_pages, page_size;
+  int32_t kv_row_width, kv_dtype;
+  int32_t num_heads, rank, rope_width, rot_dim;
+  int32_t rms_heads, rms_mode;
+  int32_t interleaved, positions_i64;
+  float scale;
+  const float* k_scale; /* device scalar, FP8 only */
+  int32_t* status;
+  int32_t device;
+} qmla_rope_cache_params;
+
+int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream);
+
 /* ---- DCP over NVLink peer memory ------------------------------------------
  * Each rank of a DCP group (one process per GPU) owns one exchange buffer:
  *   [header 256 B: flags[8] u32 (epoch published by each rank), status u32 at byte 32,

@@ -140,6 +140,73 @@ class GatherParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``qmla_rotary_params`` (field order and types must match qmla.h)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride_token", ctypes.c_int64),
+        ("x_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("num_tokens", ctypes.c_int64),
+        ("num_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("start", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("blocks", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("adjoint", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("positions", ctypes.c_void_p),
+        ("positions_i64", ctypes.c_int32),
+        ("steps", ctypes.c_void_p),
+        ("device", ctypes.c_int32),
+    ]
+
+
+class RopeCacheParams(ctypes.Structure):
+    """Mirror of ``qmla_rope_cache_params`` (field order and types must match qmla.h)."""
+
+    _fields_ = [
+        ("q_pe", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_stride_token", ctypes.c_int64),
+        ("q_out_stride_head", ctypes.c_int64),
+        ("latent", ctypes.c_void_p),
+        ("latent_stride", ctypes.c_int64),
+        ("k_pe", ctypes.c_void_p),
+        ("k_pe_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("steps", ctypes.c_void_p),
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_stride_page", ctypes.c_int64),
+        ("kv_stride_token", ctypes.c_int64),
+        ("num_tokens", ctypes.c_int64),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("kv_row_width", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("rope_width", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("rms_heads", ctypes.c_int32),
+        ("rms_mode", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("positions_i64", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("k_scale", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("device", ctypes.c_int32),
+    ]
+
+
 # device status bits (qmla_read_status / the gather's status word)
 DEV_ERR_TIMEOUT, DEV_ERR_INDEX = 1, 2
 
@@ -167,6 +234,8 @@ PROTOTYPES = {
     "qmla_dcp_p2p_merge": (ctypes.c_int, [ctypes.POINTER(DcpP2PParams), _VP]),
     "qmla_dcp_read_status": (ctypes.c_int, [_VP, _VP, ctypes.POINTER(_I32)]),
     "qmla_gather_cache": (ctypes.c_int, [ctypes.POINTER(GatherParams), _VP]),
+    "qmla_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), _VP]),
+    "qmla_rope_cache_write": (ctypes.c_int, [ctypes.POINTER(RopeCacheParams), _VP]),
 }
 
 _lib = None
