@@ -322,6 +322,49 @@ typedef struct qmla_rope_cache_params {
 
 int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream);
 
+/* ---- attention of a drafted token tree -------------------------------------
+ * Every request has ctx_lens[r] committed tokens and num_nodes (<= 64) drafted ones, whose cache
+ * rows are tokens ctx_lens[r] .. ctx_lens[r] + num_nodes - 1 of its pages.  Query row
+ * r * num_nodes + i is node i of request r; it sees the committed tokens and the drafted tokens j
+ * whose bit j is set in tree_mask[r * mask_stride + i] (itself and its ancestors; mask_stride 0:
+ * one tree for all requests).  A node whose mask is 0 is padding: o = 0, lse = -inf.  Scores,
+ * rms divisors, outputs and strides are qmla_mla_decode's.  A negative length counts as 0; tokens
+ * past block_table_cols pages, and pages outside [0, kv_num_pages), count as absent.
+ * What a hidden token's row holds, NaN included, cannot reach a node that does not see it. */
+typedef struct qmla_tree_params {
+  const void* q;
+  int64_t q_stride_row, q_stride_head;
+  const void* q_pe;
+  int64_t qpe_stride_row, qpe_stride_head;
+  int32_t q_dtype; /* QMLA_DT_BF16 or QMLA_DT_F16 */
+  const void* kv_cache;
+  int64_t kv_stride_page, kv_stride_token; /* elements; rows 16-byte aligned */
+  int64_t kv_num_pages;
+  int32_t kv_row_width, kv_dtype, page_size;
+  const int32_t* block_table; /* [num_reqs][block_table_cols] */
+  int64_t block_table_stride, block_table_cols;
+  const int32_t* ctx_lens;  /* [num_reqs] */
+  const int64_t* tree_mask; /* [num_nodes] per request */
+  int64_t mask_stride;
+  int32_t num_reqs, num_nodes, num_heads;
+  int32_t rank, qk_dim; /* <= 2048 */
+  int32_t rms_offset, rms_mode;
+  float sm_scale, logit_cap;
+  const float* k_scale; /* device scalar, FP8 (NULL = 1) */
+  void* o;
+  int64_t o_stride_row, o_stride_head;
+  int32_t o_dtype;
+  void* lse; /* may be NULL */
+  int64_t lse_stride_row;
+  int32_t lse_dtype;
+  void* workspace; /* 256-byte aligned, qmla_tree_workspace_bytes() */
+  int64_t workspace_bytes;
+  int32_t device;
+} qmla_tree_params;
+
+int qmla_tree_workspace_bytes(const qmla_tree_params* p, int64_t* bytes);
+int qmla_tree_attention(const qmla_tree_params* p, void* stream);
+
 /* ---- DCP over NVLink peer memory ------------------------------------------
  * Each rank of a DCP group (one process per GPU) owns one exchange buffer:
  *   [header 256 B: flags[8] u32 (epoch published by each rank), status u32 at byte 32,

@@ -207,6 +207,53 @@ class RopeCacheParams(ctypes.Structure):
     ]
 
 
+class TreeParams(ctypes.Structure):
+    """Mirror of ``qmla_tree_params`` (field order and types must match qmla.h)."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_row", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("q_pe", ctypes.c_void_p),
+        ("qpe_stride_row", ctypes.c_int64),
+        ("qpe_stride_head", ctypes.c_int64),
+        ("q_dtype", ctypes.c_int32),
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_stride_page", ctypes.c_int64),
+        ("kv_stride_token", ctypes.c_int64),
+        ("kv_num_pages", ctypes.c_int64),
+        ("kv_row_width", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int64),
+        ("ctx_lens", ctypes.c_void_p),
+        ("tree_mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+        ("num_reqs", ctypes.c_int32),
+        ("num_nodes", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("qk_dim", ctypes.c_int32),
+        ("rms_offset", ctypes.c_int32),
+        ("rms_mode", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("logit_cap", ctypes.c_float),
+        ("k_scale", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("o_stride_row", ctypes.c_int64),
+        ("o_stride_head", ctypes.c_int64),
+        ("o_dtype", ctypes.c_int32),
+        ("lse", ctypes.c_void_p),
+        ("lse_stride_row", ctypes.c_int64),
+        ("lse_dtype", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("device", ctypes.c_int32),
+    ]
+
+
 # device status bits (qmla_read_status / the gather's status word)
 DEV_ERR_TIMEOUT, DEV_ERR_INDEX = 1, 2
 
@@ -234,6 +281,8 @@ PROTOTYPES = {
     "qmla_dcp_p2p_merge": (ctypes.c_int, [ctypes.POINTER(DcpP2PParams), _VP]),
     "qmla_dcp_read_status": (ctypes.c_int, [_VP, _VP, ctypes.POINTER(_I32)]),
     "qmla_gather_cache": (ctypes.c_int, [ctypes.POINTER(GatherParams), _VP]),
+    "qmla_tree_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(TreeParams), ctypes.POINTER(_I64)]),
+    "qmla_tree_attention": (ctypes.c_int, [ctypes.POINTER(TreeParams), _VP]),
     "qmla_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), _VP]),
     "qmla_rope_cache_write": (ctypes.c_int, [ctypes.POINTER(RopeCacheParams), _VP]),
 }

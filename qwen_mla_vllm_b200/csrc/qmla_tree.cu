@@ -1,0 +1,413 @@
+// Attention of a drafted token tree over the paged latent cache.
+//
+// Request r has ctx committed tokens and T drafted ones whose rows sit behind them in its pages.
+// Node i sees tokens [0, ctx) and the drafted tokens of its 64-bit mask (itself and its
+// ancestors):  s = (q . k) / rms(token, head) * sm_scale,  o = softmax(s) . latent,
+// lse = ln sum exp s.  A node with an empty mask is padding: o = 0, lse = -inf.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "qmla.h"
+#include "qmla_decode.cuh"
+#include "qmla_host.cuh"
+
+using namespace qmla;
+
+namespace {
+
+constexpr int kGenThreads = 256;
+constexpr int kGenTile = 32;   // tokens per step of the generic kernel
+constexpr int kGenHeads = 8;   // heads per block of the generic kernel, one softmax warp each
+constexpr int kMaxNodes = 64;
+constexpr int kMaxRank = 2048;
+
+struct TreeArgs {
+  const uint8_t *q, *q_pe;
+  int64_t q_sr, q_sh, qpe_sr, qpe_sh;  // elements
+  int q_dtype;
+  const uint8_t* cache;
+  int64_t page_b, tok_b, num_pages;
+  const int32_t* bt;
+  int64_t bt_stride, bt_cols;
+  int page_size;
+  const int32_t* ctx;
+  const int64_t* mask;
+  int64_t mask_stride;  // elements between requests; 0: one tree for all
+  int reqs, nodes, heads, rank, qk_dim, rms_mode;
+  int64_t rms_off_b;
+  float sm_scale, logit_cap;
+  const float* k_scale;
+  uint8_t* o;
+  int64_t o_sr, o_sh;
+  int o_dtype;
+  uint8_t* lse;
+  int64_t lse_sr;
+  int lse_dtype;
+  float* part_o;    // [nsplit][rows][heads][rank]
+  float* part_lse;  // [nsplit][rows][heads], log2 units
+  int nsplit;
+};
+
+// Committed tokens of request r, clamped to what its block-table row can hold.
+__device__ __forceinline__ int tree_ctx(const TreeArgs& a, int r) {
+  const int64_t room = a.bt_cols * a.page_size;
+  return (int)min((int64_t)max(__ldg(a.ctx + r), 0), room);
+}
+
+// 1 / rms(token, head) of a cache row; a divisor that is not positive counts as 1.
+template <bool FP8>
+__device__ __forceinline__ float inv_rms(const TreeArgs& a, const uint8_t* row, int h, float kscale) {
+  if (a.rms_mode == QMLA_RMS_NONE) return 1.f;
+  const uint8_t* p = row + a.rms_off_b;
+  if (FP8 && a.rms_mode == QMLA_RMS_LOG8) return ex2_approx(3.0f - (float)__ldg(p + h) * (6.0f / 255.0f));
+  float rv;
+  if (!FP8)
+    rv = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[h]);
+  else if (a.rms_mode == QMLA_RMS_BF16)  // raw bytes: the offset may be odd
+    rv = __bfloat162float(__ushort_as_bfloat16((uint16_t)(__ldg(p + 2 * h) | (__ldg(p + 2 * h + 1) << 8))));
+  else
+    rv = e4m3_to_f32(__ldg(p + h)) * kscale;
+  return rv > 0.f ? 1.f / rv : 1.f;
+}
+
+// ---------------------------------------------------------------- generic kernel
+// Any rank, page size and head count; 32-bit arithmetic on the CUDA cores.  One block per
+// (node, 8 heads, split of the tokens).  Per 32-token step: each warp scores 4 tokens against the
+// 8 heads (a lane takes a 16-byte unit of the key row), then warp h updates head h's running
+// maximum and sum, then every thread adds the visible tokens' values to its output dims.  Values of
+// tokens that the node does not see are not read, so what they hold cannot matter.
+template <bool FP8>
+__global__ void __launch_bounds__(kGenThreads) tree_generic_kernel(const TreeArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int V = FP8 ? 16 : 8;  // elements per 16-byte unit
+  const int units = (a.qk_dim + V - 1) / V;
+  float* qs = reinterpret_cast<float*>(smem);  // [8][units * V], zero past qk_dim
+  const int qst = units * V;
+  __shared__ float s_s[kGenTile][kGenHeads];
+  __shared__ float p_s[kGenTile][kGenHeads];
+  __shared__ float alpha_s[kGenHeads], l_s[kGenHeads];
+  __shared__ const uint8_t* rows_s[kGenTile];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hgroups = (a.heads + kGenHeads - 1) / kGenHeads;
+  const int row = blockIdx.x / hgroups, h0 = (blockIdx.x - row * hgroups) * kGenHeads;
+  const int nh = min(kGenHeads, a.heads - h0);
+  const int r = row / a.nodes, node = row - r * a.nodes;
+  const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
+  const uint64_t mask = (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + r * a.mask_stride + node);
+  const int ctx = tree_ctx(a, r);
+  // tokens this node may see: up to its last visible draft
+  int64_t n = mask ? (int64_t)ctx + 64 - __clzll((long long)mask) : 0;
+  n = min(n, min(a.bt_cols * a.page_size, (int64_t)ctx + a.nodes));
+  const int64_t tiles = (n + kGenTile - 1) / kGenTile;
+  const int64_t t_lo = tiles * blockIdx.y / a.nsplit, t_hi = tiles * (blockIdx.y + 1) / a.nsplit;
+  for (int i = tid; i < kGenHeads * qst; i += kGenThreads) {
+    const int h = i / qst, d = i - h * qst;
+    float v = 0.f;
+    if (h < nh && d < a.qk_dim) {
+      const uint8_t* src = d < a.rank ? a.q + ((int64_t)row * a.q_sr + (int64_t)(h0 + h) * a.q_sh + d) * 2
+                                      : a.q_pe + ((int64_t)row * a.qpe_sr + (int64_t)(h0 + h) * a.qpe_sh + d - a.rank) * 2;
+      v = load_as_float(src, a.q_dtype);
+    }
+    qs[i] = v;
+  }
+  float acc[kMaxRank / kGenThreads][kGenHeads];
+#pragma unroll
+  for (int k = 0; k < kMaxRank / kGenThreads; ++k)
+#pragma unroll
+    for (int h = 0; h < kGenHeads; ++h) acc[k][h] = 0.f;
+  float m = -INFINITY, l = 0.f;  // warp h: head h0 + h
+  __syncthreads();
+  for (int64_t t = t_lo; t < t_hi; ++t) {
+    const int64_t tok0 = t * kGenTile;
+    for (int j = warp; j < kGenTile; j += kGenThreads / 32) {
+      const int64_t tok = tok0 + j;
+      bool see = tok < n;
+      if (see && tok >= ctx) see = mask >> (tok - ctx) & 1;
+      const uint8_t* kr = nullptr;
+      if (see) {
+        const int pg = __ldg(a.bt + r * a.bt_stride + tok / a.page_size);
+        if (pg >= 0 && pg < a.num_pages)
+          kr = a.cache + (int64_t)pg * a.page_b + tok % a.page_size * a.tok_b;
+        see = kr != nullptr;  // a page id outside the cache: the token counts as absent
+      }
+      float d[kGenHeads];
+#pragma unroll
+      for (int h = 0; h < kGenHeads; ++h) d[h] = 0.f;
+      if (see) {
+        for (int u = lane; u < units; u += 32) {
+          alignas(16) uint8_t raw[16];
+          *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(kr) + u);
+          float kv[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float x = FP8 ? e4m3_to_f32(raw[e]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(raw)[e]);
+            kv[e] = u * V + e < a.qk_dim ? x : 0.f;  // the unit may run into the rms tail
+          }
+#pragma unroll
+          for (int h = 0; h < kGenHeads; ++h) {
+            const float4* q4 = reinterpret_cast<const float4*>(qs + h * qst + u * V);
+#pragma unroll
+            for (int e = 0; e < V / 4; ++e) {
+              const float4 qv = q4[e];
+              d[h] += qv.x * kv[4 * e] + qv.y * kv[4 * e + 1] + qv.z * kv[4 * e + 2] + qv.w * kv[4 * e + 3];
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < kGenHeads; ++h)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) d[h] += __shfl_xor_sync(0xffffffffu, d[h], o);
+      if (lane < kGenHeads) {
+        float x = -INFINITY;
+        if (see && lane < nh) {
+          float dh = d[0];
+#pragma unroll
+          for (int h = 1; h < kGenHeads; ++h) dh = lane == h ? d[h] : dh;
+          x = dh * kscale * inv_rms<FP8>(a, kr, h0 + lane, kscale) * a.sm_scale;
+          if (a.logit_cap > 0.f) x = a.logit_cap * tanhf(x / a.logit_cap);
+          x *= kLog2e;
+        }
+        s_s[j][lane] = x;
+      }
+      if (lane == 0) rows_s[j] = see ? kr : nullptr;
+    }
+    __syncthreads();
+    {
+      const float x = s_s[lane][warp];
+      float mx = x;
+      bool bad = x != x;  // fmaxf drops a NaN: carry it into the sum instead
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(m, mx);
+      const float al = m == mn ? 1.f : exp2f(m - mn);
+      float p = bad ? x : (x == -INFINITY ? 0.f : exp2f(x - mn));
+      p_s[lane][warp] = p;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o);
+      l = l * al + p;
+      m = mn;
+      if (lane == 0) alpha_s[warp] = al;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMaxRank / kGenThreads; ++k) {
+      const int dcol = tid + k * kGenThreads;
+      if (dcol < a.rank) {
+#pragma unroll
+        for (int h = 0; h < kGenHeads; ++h) acc[k][h] *= alpha_s[h];
+        for (int j = 0; j < kGenTile; ++j) {
+          const uint8_t* kr = rows_s[j];
+          if (!kr) continue;
+          const float v = FP8 ? e4m3_to_f32(__ldg(kr + dcol)) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(kr)[dcol]);
+#pragma unroll
+          for (int h = 0; h < kGenHeads; ++h) acc[k][h] += p_s[j][h] * v;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (lane == 0) {
+    alpha_s[warp] = m;
+    l_s[warp] = l;
+  }
+  __syncthreads();
+  const int64_t prow = ((int64_t)blockIdx.y * a.reqs * a.nodes + row) * a.heads + h0;
+  for (int h = 0; h < nh; ++h) {
+    const float lt = l_s[h];
+    const float inv = lt == 0.f ? 0.f : kscale / lt;
+#pragma unroll
+    for (int k = 0; k < kMaxRank / kGenThreads; ++k) {
+      const int dcol = tid + k * kGenThreads;
+      if (dcol >= a.rank) continue;
+      float v = acc[k][0];
+#pragma unroll
+      for (int g = 1; g < kGenHeads; ++g) v = g == h ? acc[k][g] : v;
+      v *= inv;
+      if (a.nsplit == 1)
+        store_from_float(a.o + ((int64_t)row * a.o_sr + (int64_t)(h0 + h) * a.o_sh + dcol) * dt_size(a.o_dtype), a.o_dtype, v);
+      else
+        a.part_o[(prow + h) * a.rank + dcol] = v;
+    }
+  }
+  if (tid < nh) {
+    const float l2 = alpha_s[tid] + log2f(l_s[tid]);  // -inf where nothing is visible
+    if (a.nsplit > 1)
+      a.part_lse[prow + tid] = l2;
+    else if (a.lse)
+      store_from_float(a.lse + ((int64_t)row * a.lse_sr + h0 + tid) * dt_size(a.lse_dtype), a.lse_dtype, l2 * kLn2);
+  }
+}
+
+// Joins the splits of a (row, head): o = sum_i 2^(lse_i - lse) o_i.  Splits without tokens carry
+// lse = -inf and are not read; a NaN of any split is a NaN of the result.
+__global__ void __launch_bounds__(128) tree_join_kernel(const TreeArgs a) {
+  const int64_t rh = blockIdx.x;
+  const int64_t n = (int64_t)a.reqs * a.nodes * a.heads;
+  const int64_t row = rh / a.heads;
+  const int h = (int)(rh - row * a.heads);
+  float m = -INFINITY;
+  bool bad = false;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float l = __ldg(a.part_lse + s * n + rh);
+    m = fmaxf(m, l);
+    bad |= l != l;
+  }
+  float sum = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float l = __ldg(a.part_lse + s * n + rh);
+    sum += l == -INFINITY ? 0.f : exp2f(l - m);
+  }
+  if (bad) sum = NAN;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint8_t* orow = a.o + (row * a.o_sr + (int64_t)h * a.o_sh) * dt_size(a.o_dtype);
+  for (int d = threadIdx.x; d < a.rank; d += blockDim.x) {
+    float acc = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float l = __ldg(a.part_lse + s * n + rh);
+      if (l != -INFINITY) acc += exp2f(l - m) * __ldg(a.part_o + (s * n + rh) * a.rank + d);
+    }
+    store_from_float(orow + (int64_t)d * dt_size(a.o_dtype), a.o_dtype, acc * inv);
+  }
+  if (threadIdx.x == 0 && a.lse)
+    store_from_float(a.lse + (row * a.lse_sr + h) * dt_size(a.lse_dtype), a.lse_dtype, (m + log2f(sum)) * kLn2);
+}
+
+struct TreePlan {
+  int nsplit;
+  int64_t ws_lse, ws_o, ws_total;
+};
+
+int make_tree_plan(const qmla_tree_params* p, TreePlan* pl) {
+  if (!p || p->num_reqs < 0 || p->num_nodes < 0 || p->num_heads <= 0 || p->rank <= 0 || p->qk_dim < p->rank ||
+      p->page_size <= 0 || p->kv_num_pages < 0 || p->block_table_cols < 0)
+    return QMLA_E_INVALID;
+  if (p->num_nodes > kMaxNodes || p->rank > kMaxRank || p->qk_dim > kMaxRank) return QMLA_E_UNSUPPORTED;
+  if (p->q_dtype != QMLA_DT_BF16 && p->q_dtype != QMLA_DT_F16) return QMLA_E_UNSUPPORTED;
+  if (p->o_dtype < 0 || p->o_dtype > 2 || p->lse_dtype < 0 || p->lse_dtype > 2) return QMLA_E_UNSUPPORTED;
+  const bool fp8 = p->kv_dtype == QMLA_DT_FP8E4M3;
+  if (!fp8 && p->kv_dtype != QMLA_DT_BF16) return QMLA_E_UNSUPPORTED;
+  if (p->rms_mode < 0 || p->rms_mode > 3 || (!fp8 && p->rms_mode >= 2)) return QMLA_E_INVALID;
+  const int es = fp8 ? 1 : 2;
+  if (reinterpret_cast<uintptr_t>(p->kv_cache) % 16 != 0 || p->kv_stride_token * es % 16 != 0 ||
+      p->kv_stride_page * es % 16 != 0)
+    return QMLA_E_ALIGNMENT;
+  if (p->kv_row_width < p->qk_dim || p->kv_stride_token < p->kv_row_width) return QMLA_E_INVALID;
+  if (p->rms_mode != QMLA_RMS_NONE) {
+    const int64_t tail = (int64_t)p->num_heads * (fp8 && p->rms_mode == QMLA_RMS_BF16 ? 2 : 1);
+    if (p->rms_offset < p->qk_dim || p->rms_offset + tail > p->kv_row_width) return QMLA_E_INVALID;
+  }
+  const DevInfo di = dev_info(p->device);
+  if (!di.ok) return QMLA_E_CUDA;
+  const int64_t rows = (int64_t)p->num_reqs * p->num_nodes;
+  const int64_t blocks = rows * ((p->num_heads + kGenHeads - 1) / kGenHeads);
+  if (blocks > INT32_MAX || rows * p->num_heads > INT32_MAX) return QMLA_E_UNSUPPORTED;
+  // tokens split over blocks until every SM has two
+  pl->nsplit = blocks == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(64, 2 * di.sms / blocks));
+  int64_t w = 0;
+  pl->ws_lse = w;
+  if (pl->nsplit > 1) w = align_up(w + 4 * rows * p->num_heads * pl->nsplit, 256);
+  pl->ws_o = w;
+  if (pl->nsplit > 1) w = align_up(w + 4 * rows * p->num_heads * p->rank * pl->nsplit, 256);
+  pl->ws_total = w;
+  return QMLA_OK;
+}
+
+template <bool FP8>
+int launch_generic(const TreeArgs& a, cudaStream_t st) {
+  const int V = FP8 ? 16 : 8;
+  const int smem = kGenHeads * ((a.qk_dim + V - 1) / V * V) * 4;
+  static std::once_flag once;
+  static cudaError_t err = cudaSuccess;
+  std::call_once(once, [] {
+    err = cudaFuncSetAttribute(tree_generic_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kGenHeads * kMaxRank * 4);
+  });
+  if (err != cudaSuccess) return QMLA_E_CUDA;
+  const int hgroups = (a.heads + kGenHeads - 1) / kGenHeads;
+  tree_generic_kernel<FP8><<<dim3(a.reqs * a.nodes * hgroups, a.nsplit), kGenThreads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qmla_tree_workspace_bytes(const qmla_tree_params* p, int64_t* bytes) {
+  if (!bytes) return QMLA_E_INVALID;
+  TreePlan pl;
+  const int rc = make_tree_plan(p, &pl);
+  if (rc != QMLA_OK) return rc;
+  *bytes = pl.ws_total;
+  return QMLA_OK;
+}
+
+int qmla_tree_attention(const qmla_tree_params* p, void* stream) {
+  TreePlan pl;
+  int rc = make_tree_plan(p, &pl);
+  if (rc != QMLA_OK) return rc;
+  if (p->num_reqs == 0 || p->num_nodes == 0) return QMLA_OK;
+  if (!p->q || (!p->q_pe && p->qk_dim > p->rank) || !p->kv_cache || !p->block_table || !p->ctx_lens ||
+      !p->tree_mask || !p->o)
+    return QMLA_E_INVALID;
+  if (pl.ws_total > 0) {
+    if (!p->workspace || p->workspace_bytes < pl.ws_total) return QMLA_E_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(p->workspace) % 256 != 0) return QMLA_E_ALIGNMENT;
+  }
+  DeviceGuard dg(p->device);
+  if (!dg.ok()) return QMLA_E_CUDA;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool fp8 = p->kv_dtype == QMLA_DT_FP8E4M3;
+  const int es = fp8 ? 1 : 2;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(p->workspace);
+  TreeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = reinterpret_cast<const uint8_t*>(p->q);
+  a.q_pe = reinterpret_cast<const uint8_t*>(p->q_pe ? p->q_pe : p->q);
+  a.q_sr = p->q_stride_row;
+  a.q_sh = p->q_stride_head;
+  a.qpe_sr = p->qpe_stride_row;
+  a.qpe_sh = p->qpe_stride_head;
+  a.q_dtype = p->q_dtype;
+  a.cache = reinterpret_cast<const uint8_t*>(p->kv_cache);
+  a.page_b = p->kv_stride_page * es;
+  a.tok_b = p->kv_stride_token * es;
+  a.num_pages = p->kv_num_pages;
+  a.bt = p->block_table;
+  a.bt_stride = p->block_table_stride;
+  a.bt_cols = p->block_table_cols;
+  a.page_size = p->page_size;
+  a.ctx = p->ctx_lens;
+  a.mask = p->tree_mask;
+  a.mask_stride = p->mask_stride;
+  a.reqs = p->num_reqs;
+  a.nodes = p->num_nodes;
+  a.heads = p->num_heads;
+  a.rank = p->rank;
+  a.qk_dim = p->qk_dim;
+  a.rms_mode = p->rms_mode;
+  a.rms_off_b = (int64_t)p->rms_offset * es;
+  a.sm_scale = p->sm_scale;
+  a.logit_cap = p->logit_cap;
+  a.k_scale = p->k_scale;
+  a.o = reinterpret_cast<uint8_t*>(p->o);
+  a.o_sr = p->o_stride_row;
+  a.o_sh = p->o_stride_head;
+  a.o_dtype = p->o_dtype;
+  a.lse = reinterpret_cast<uint8_t*>(p->lse);
+  a.lse_sr = p->lse_stride_row;
+  a.lse_dtype = p->lse_dtype;
+  a.part_lse = reinterpret_cast<float*>(ws + pl.ws_lse);
+  a.part_o = reinterpret_cast<float*>(ws + pl.ws_o);
+  a.nsplit = pl.nsplit;
+  rc = fp8 ? launch_generic<true>(a, st) : launch_generic<false>(a, st);
+  if (rc != QMLA_OK) return rc;
+  if (a.nsplit > 1) tree_join_kernel<<<a.reqs * a.nodes * a.heads, 128, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+}
+
+}  // extern "C"

@@ -14,7 +14,8 @@ from test_abi import shutil
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
 @pytest.mark.parametrize("cname,pystruct", [("qmla_rotary_params", _lib.RotaryParams),
-                                            ("qmla_rope_cache_params", _lib.RopeCacheParams)])
+                                            ("qmla_rope_cache_params", _lib.RopeCacheParams),
+                                            ("qmla_tree_params", _lib.TreeParams)])
 def test_struct_layout(tmp_path, cname, pystruct):
     check_layout(tmp_path, cname, pystruct)
 
