@@ -365,6 +365,79 @@ typedef struct qmla_tree_params {
 int qmla_tree_workspace_bytes(const qmla_tree_params* p, int64_t* bytes);
 int qmla_tree_attention(const qmla_tree_params* p, void* stream);
 
+/* ---- accumulated attention weight, and eviction by it ----------------------
+ * For every request r and token t before the longest of its qrows row lengths:
+ *   weights[r][t] = decay * weights[r][t] + sum_{j, h} exp(s_jht - lse[r * qrows + j][h])
+ * over the query rows j with t < seq_lens[r * qrows + j], scores as qmla_mla_decode's, lse (natural
+ * log) as it returns for the same rows.  Rows whose lse is not finite add nothing; tokens of
+ * pages outside [0, kv_num_pages) only decay; other columns are left as they are.  Each weight has
+ * one writer and a fixed order of summation. */
+typedef struct qmla_weights_params {
+  const void* q; /* rows r * qrows + j */
+  int64_t q_stride_row, q_stride_head;
+  const void* q_pe;
+  int64_t qpe_stride_row, qpe_stride_head;
+  int32_t q_dtype; /* QMLA_DT_BF16 or QMLA_DT_F16 */
+  const void* kv_cache;
+  int64_t kv_stride_page, kv_stride_token; /* elements; rows 16-byte aligned */
+  int64_t kv_num_pages;
+  int32_t kv_row_width, kv_dtype, page_size;
+  const int32_t* block_table; /* [num_reqs][block_table_cols] */
+  int64_t block_table_stride, block_table_cols;
+  const int32_t* seq_lens; /* [num_reqs * qrows] */
+  int32_t num_reqs, qrows, num_heads;
+  int32_t rank, qk_dim; /* <= 2048 */
+  int32_t rms_offset, rms_mode;
+  float sm_scale, logit_cap, decay;
+  const float* k_scale; /* device scalar, FP8 (NULL = 1) */
+  const float* lse;     /* [num_reqs * qrows][num_heads] */
+  int64_t lse_stride_row;
+  float* weights; /* [num_reqs][weights_cols] */
+  int64_t weights_stride_req, weights_cols;
+  void* workspace; /* 256-byte aligned, qmla_weights_workspace_bytes() */
+  int64_t workspace_bytes;
+  int32_t device;
+} qmla_weights_params;
+
+int qmla_weights_workspace_bytes(const qmla_weights_params* p, int64_t* bytes);
+int qmla_accumulate_weights(const qmla_weights_params* p, void* stream);
+
+/* Keep the K = min(n, budget, budgets[r]) heaviest of request r's n = seq_lens[r] tokens, and
+ * close up the cache.  Tokens whose position is below `sinks` or at or past recent_from[r] come
+ * before all others, then the larger weight (NaN last), then the lower index.  The i-th kept token at
+ * or past K moves, row and all, into the i-th place below K that was given up; every other kept
+ * token stays where it is.  new_weights / new_positions [num_reqs][new_cols] get the tokens' weights
+ * and positions in their new places, 0 and -1 past K; new_lens gets K.  The outputs must not overlap
+ * the inputs, and a request's pages must be its own (not shared with another's prefix). */
+typedef struct qmla_evict_params {
+  void* kv_cache; /* any row format: row_bytes are moved */
+  int64_t page_stride_bytes, token_stride_bytes, row_bytes, kv_num_pages;
+  int32_t page_size;
+  const int32_t* block_table;
+  int64_t block_table_stride, block_table_cols;
+  const float* weights;
+  int64_t weights_stride_req;
+  const int32_t* positions;
+  int64_t positions_stride_req;
+  int64_t cols; /* columns of weights and positions */
+  const int32_t* seq_lens;
+  const int32_t* budgets; /* per request, or NULL */
+  int32_t budget;
+  int32_t sinks;
+  const int32_t* recent_from; /* per request, or NULL */
+  float* new_weights;
+  int32_t* new_positions;
+  int64_t new_stride_req, new_cols; /* >= min(budget, cols) */
+  int32_t* new_lens;
+  int32_t num_reqs;
+  void* workspace; /* 256-byte aligned, qmla_evict_workspace_bytes() */
+  int64_t workspace_bytes;
+  int32_t device;
+} qmla_evict_params;
+
+int qmla_evict_workspace_bytes(const qmla_evict_params* p, int64_t* bytes);
+int qmla_evict(const qmla_evict_params* p, void* stream);
+
 /* ---- DCP over NVLink peer memory ------------------------------------------
  * Each rank of a DCP group (one process per GPU) owns one exchange buffer:
  *   [header 256 B: flags[8] u32 (epoch published by each rank), status u32 at byte 32,

@@ -254,6 +254,85 @@ class TreeParams(ctypes.Structure):
     ]
 
 
+class WeightsParams(ctypes.Structure):
+    """Mirror of ``qmla_weights_params`` (field order and types must match qmla.h)."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_row", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("q_pe", ctypes.c_void_p),
+        ("qpe_stride_row", ctypes.c_int64),
+        ("qpe_stride_head", ctypes.c_int64),
+        ("q_dtype", ctypes.c_int32),
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_stride_page", ctypes.c_int64),
+        ("kv_stride_token", ctypes.c_int64),
+        ("kv_num_pages", ctypes.c_int64),
+        ("kv_row_width", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("num_reqs", ctypes.c_int32),
+        ("qrows", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("qk_dim", ctypes.c_int32),
+        ("rms_offset", ctypes.c_int32),
+        ("rms_mode", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("logit_cap", ctypes.c_float),
+        ("decay", ctypes.c_float),
+        ("k_scale", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("lse_stride_row", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("weights_stride_req", ctypes.c_int64),
+        ("weights_cols", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("device", ctypes.c_int32),
+    ]
+
+
+class EvictParams(ctypes.Structure):
+    """Mirror of ``qmla_evict_params`` (field order and types must match qmla.h)."""
+
+    _fields_ = [
+        ("kv_cache", ctypes.c_void_p),
+        ("page_stride_bytes", ctypes.c_int64),
+        ("token_stride_bytes", ctypes.c_int64),
+        ("row_bytes", ctypes.c_int64),
+        ("kv_num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("weights_stride_req", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("positions_stride_req", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("budgets", ctypes.c_void_p),
+        ("budget", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("recent_from", ctypes.c_void_p),
+        ("new_weights", ctypes.c_void_p),
+        ("new_positions", ctypes.c_void_p),
+        ("new_stride_req", ctypes.c_int64),
+        ("new_cols", ctypes.c_int64),
+        ("new_lens", ctypes.c_void_p),
+        ("num_reqs", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("device", ctypes.c_int32),
+    ]
+
+
 # device status bits (qmla_read_status / the gather's status word)
 DEV_ERR_TIMEOUT, DEV_ERR_INDEX = 1, 2
 
@@ -283,6 +362,10 @@ PROTOTYPES = {
     "qmla_gather_cache": (ctypes.c_int, [ctypes.POINTER(GatherParams), _VP]),
     "qmla_tree_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(TreeParams), ctypes.POINTER(_I64)]),
     "qmla_tree_attention": (ctypes.c_int, [ctypes.POINTER(TreeParams), _VP]),
+    "qmla_weights_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(WeightsParams), ctypes.POINTER(_I64)]),
+    "qmla_accumulate_weights": (ctypes.c_int, [ctypes.POINTER(WeightsParams), _VP]),
+    "qmla_evict_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(EvictParams), ctypes.POINTER(_I64)]),
+    "qmla_evict": (ctypes.c_int, [ctypes.POINTER(EvictParams), _VP]),
     "qmla_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), _VP]),
     "qmla_rope_cache_write": (ctypes.c_int, [ctypes.POINTER(RopeCacheParams), _VP]),
 }

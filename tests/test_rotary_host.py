@@ -15,7 +15,9 @@ from test_abi import shutil
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
 @pytest.mark.parametrize("cname,pystruct", [("qmla_rotary_params", _lib.RotaryParams),
                                             ("qmla_rope_cache_params", _lib.RopeCacheParams),
-                                            ("qmla_tree_params", _lib.TreeParams)])
+                                            ("qmla_tree_params", _lib.TreeParams),
+                                            ("qmla_weights_params", _lib.WeightsParams),
+                                            ("qmla_evict_params", _lib.EvictParams)])
 def test_struct_layout(tmp_path, cname, pystruct):
     check_layout(tmp_path, cname, pystruct)
 
