@@ -48,6 +48,18 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// Tiled map over 2-byte (bf16) or 1-byte elements, 128-byte swizzle; dims[0] is dense, strides in
+// bytes are those of dims[1..].  False when the driver refuses it.
+inline bool encode_tiled(CUtensorMap* m, bool fp8, const void* base, int nd, const cuuint64_t* dims,
+                         const cuuint64_t* strides, const cuuint32_t* box) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(m, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, nd, const_cast<void*>(base), dims,
+            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 inline int gcd_int(int a, int b) {
   while (b) {
     int t = a % b;

@@ -1,0 +1,89 @@
+// Query rows as the tensor cores read them: K-major operand images with the 128-byte swizzle,
+// written to the workspace once per call so that a kernel stages a whole image with bulk copies.
+//
+// An image holds `nrows` rows (a multiple of 8) of `chunks` 128-byte columns, term by term:
+//   byte (term, chunk, row, b) = term * term_bytes + chunk * nrows * 128 + row * 128 + (b ^ ((row & 7) << 4))
+// A query element is a sum of up to three terms of the cache's element type, each the rounding of what
+// the ones before it leave:
+//   bf16 cache: a bf16 query is one term, an f16 query two (8 + 8 bits hold its 11);
+//   FP8 cache:  e4m3 has 4 significant bits, so a bf16 query takes two terms and an f16 query three,
+//               after a scaling by the power of two that brings the row's largest element into
+//               (224, 448].  What is lost is below 2^-10 of that scale: 2^-17 of the largest element.
+// The scaling is undone where the scores are (q_scale holds its inverse).
+#pragma once
+#include "qmla_decode.cuh"
+
+namespace qmla {
+
+inline int q_terms(bool fp8, int q_dtype) { return (fp8 ? 2 : 1) + (q_dtype == 1 ? 1 : 0); }
+
+struct QSource {
+  const uint8_t *q, *q_pe;
+  int64_t q_sr, q_sh, qpe_sr, qpe_sh;  // elements
+  int dtype;
+  int rank, qk_dim;
+};
+
+// Writes one row (all terms) of an image; src_row < 0 writes zeros.  One warp.  Returns the inverse
+// of the row's scaling in every lane.
+template <bool FP8>
+__device__ __forceinline__ float write_q_row(const QSource& s, int64_t src_row, int head, uint8_t* img, int row,
+                                             int nrows, int chunks, int terms) {
+  constexpr int V = FP8 ? 16 : 8;  // elements of a 16-byte unit
+  const int lane = threadIdx.x & 31;
+  const int units = chunks * 8;
+  const int64_t term_bytes = (int64_t)chunks * nrows * 128;
+  auto elem = [&](int d) -> float {
+    if (src_row < 0 || d >= s.qk_dim) return 0.f;
+    return load_as_float(d < s.rank ? s.q + (src_row * s.q_sr + (int64_t)head * s.q_sh + d) * 2
+                                    : s.q_pe + (src_row * s.qpe_sr + (int64_t)head * s.qpe_sh + d - s.rank) * 2,
+                         s.dtype);
+  };
+  float scale = 1.f;
+  if constexpr (FP8) {
+    float mx = 0.f;
+    for (int d = lane; d < s.qk_dim; d += 32) {
+      const float v = fabsf(elem(d));
+      if (v <= 3.0e38f) mx = fmaxf(mx, v);  // finite ones
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (mx > 0.f) {
+      const int e = max(-100, min(100, (int)floorf(log2f(448.f / mx))));
+      scale = exp2f((float)e);
+      if (mx * scale > 448.f) scale *= 0.5f;  // log2f may round up to a whole number
+    }
+  }
+  for (int u = lane; u < units; u += 32) {
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = elem(u * V + e) * scale;
+    const int64_t at = (int64_t)(u >> 3) * nrows * 128 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
+    for (int t = 0; t < terms; ++t) {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if constexpr (FP8) {
+          const uint8_t b = fabsf(v[e]) <= 448.f ? f32_to_e4m3(v[e]) : 0x7f;  // not finite: NaN
+          w[e >> 2] |= (uint32_t)b << (8 * (e & 3));
+          v[e] -= e4m3_to_f32(b);
+        } else {
+          const __nv_bfloat16 b = __float2bfloat16_rn(v[e]);
+          w[e >> 1] |= (uint32_t)__bfloat16_as_ushort(b) << (16 * (e & 1));
+          v[e] = isfinite(v[e]) ? v[e] - __bfloat162float(b) : 0.f;
+        }
+      }
+      *reinterpret_cast<uint4*>(img + t * term_bytes + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  return 1.f / scale;
+}
+
+// Byte range of an image as bulk copies of at most 32 KB onto one barrier (its bytes are armed
+// by the caller): one lane.
+__device__ __forceinline__ void load_image(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar,
+                                           uint64_t policy) {
+  for (uint32_t o = 0; o < bytes; o += 32768u) bulk_load_1d(dst + o, src + o, min(32768u, bytes - o), bar, policy);
+}
+
+}  // namespace qmla
