@@ -6,16 +6,29 @@
 // A query element is a sum of up to three terms of the cache's element type, each the rounding of what
 // the ones before it leave:
 //   bf16 cache: a bf16 query is one term, an f16 query two (8 + 8 bits hold its 11);
-//   FP8 cache:  e4m3 has 4 significant bits, so a bf16 query takes two terms and an f16 query three,
-//               after a scaling by the power of two that brings the row's largest element into
-//               (224, 448].  What is lost is below 2^-10 of that scale: 2^-17 of the largest element.
-// The scaling is undone where the scores are (q_scale holds its inverse).
+//   FP8 cache:  an e4m3 term (4 significant bits) and e5m2 terms (3 bits, down to 2^-16), after a
+//               scaling by the power of two that brings the row's largest element into (224, 448].
+//               Rounding to nearest leaves a remainder that one e5m2 term holds exactly for a bf16
+//               query and two for an f16 query, as long as the e4m3 term is normal: down to 2^-15 of the
+//               row's largest element.  Below that an element is off by at most 2^-13 of the scale,
+//               2^-21 of the largest element.
+// The scaling is undone where the scores are (the caller keeps its inverse).
 #pragma once
 #include "qmla_decode.cuh"
 
 namespace qmla {
 
 inline int q_terms(bool fp8, int q_dtype) { return (fp8 ? 2 : 1) + (q_dtype == 1 ? 1 : 0); }
+
+// Formats of the terms in a kind::f8f6f4 instruction descriptor.
+__device__ __forceinline__ uint32_t q_term_format(int term) { return term == 0 ? 0u : 1u; }
+
+__device__ __forceinline__ uint8_t f32_to_e5m2(float x) {
+  return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E5M2);
+}
+__device__ __forceinline__ float e5m2_to_f32(uint8_t b) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E5M2)));
+}
 
 struct QSource {
   const uint8_t *q, *q_pe;
@@ -64,9 +77,10 @@ __device__ __forceinline__ float write_q_row(const QSource& s, int64_t src_row, 
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         if constexpr (FP8) {
-          const uint8_t b = fabsf(v[e]) <= 448.f ? f32_to_e4m3(v[e]) : 0x7f;  // not finite: NaN
+          const bool fin = fabsf(v[e]) <= 448.f;  // not finite: NaN
+          const uint8_t b = !fin ? 0x7f : t == 0 ? f32_to_e4m3(v[e]) : f32_to_e5m2(v[e]);
           w[e >> 2] |= (uint32_t)b << (8 * (e & 3));
-          v[e] -= e4m3_to_f32(b);
+          v[e] -= t == 0 ? e4m3_to_f32(b) : e5m2_to_f32(b);
         } else {
           const __nv_bfloat16 b = __float2bfloat16_rn(v[e]);
           w[e >> 1] |= (uint32_t)__bfloat16_as_ushort(b) << (16 * (e & 1));

@@ -10,10 +10,13 @@
 
 #include <algorithm>
 #include <cstring>
+#include <map>
+#include <mutex>
 
 #include "qmla.h"
 #include "qmla_decode.cuh"
 #include "qmla_host.cuh"
+#include "qmla_tree_mma.cuh"
 
 using namespace qmla;
 
@@ -24,39 +27,6 @@ constexpr int kGenTile = 32;   // tokens per step of the generic kernel
 constexpr int kGenHeads = 8;   // heads per block of the generic kernel, one softmax warp each
 constexpr int kMaxNodes = 64;
 constexpr int kMaxRank = 2048;
-
-struct TreeArgs {
-  const uint8_t *q, *q_pe;
-  int64_t q_sr, q_sh, qpe_sr, qpe_sh;  // elements
-  int q_dtype;
-  const uint8_t* cache;
-  int64_t page_b, tok_b, num_pages;
-  const int32_t* bt;
-  int64_t bt_stride, bt_cols;
-  int page_size;
-  const int32_t* ctx;
-  const int64_t* mask;
-  int64_t mask_stride;  // elements between requests; 0: one tree for all
-  int reqs, nodes, heads, rank, qk_dim, rms_mode;
-  int64_t rms_off_b;
-  float sm_scale, logit_cap;
-  const float* k_scale;
-  uint8_t* o;
-  int64_t o_sr, o_sh;
-  int o_dtype;
-  uint8_t* lse;
-  int64_t lse_sr;
-  int lse_dtype;
-  float* part_o;    // [nsplit][rows][heads][rank]
-  float* part_lse;  // [nsplit][rows][heads], log2 units
-  int nsplit;
-};
-
-// Committed tokens of request r, clamped to what its block-table row can hold.
-__device__ __forceinline__ int tree_ctx(const TreeArgs& a, int r) {
-  const int64_t room = a.bt_cols * a.page_size;
-  return (int)min((int64_t)max(__ldg(a.ctx + r), 0), room);
-}
 
 // 1 / rms(token, head) of a cache row; a divisor that is not positive counts as 1.
 template <bool FP8>
@@ -278,9 +248,99 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeArgs a) {
 }
 
 struct TreePlan {
-  int nsplit;
+  int nsplit;                     // generic kernel
   int64_t ws_lse, ws_o, ws_total;
+  bool mma;                       // tensor-core kernel
+  TreeMma m;
+  uint32_t smem;
+  int64_t ws_status, ws_prefix, ws_bounds, ws_img, ws_qinv, ws_tail;
 };
+
+// Clusters of the tensor-core kernel that can be resident at once (asked once per device).
+template <bool FP8>
+int resident_clusters(int device) {
+  static std::mutex mu;
+  static std::map<int, int> known;
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = known.find(device);
+  if (it != known.end()) return it->second;
+  int n = 0;
+  if (cudaFuncSetAttribute(tree_mma_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem) == cudaSuccess) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(kTrThreads);
+    cfg.dynamicSmemBytes = kMaxDynSmem;
+    if (cudaOccupancyMaxActiveClusters(&n, tree_mma_kernel<FP8>, &cfg) != cudaSuccess) n = 0;
+  }
+  known[device] = n;
+  return n;
+}
+
+// The tensor-core kernel takes ranks of whole 128-dim columns up to 768, pages of whole 16-token runs,
+// divisors within whole 16-byte units of the row, a query image that leaves room for three K / V
+// slots, and no more groups of 128 query rows than there are clusters.  Everything else is the
+// generic kernel's.
+void plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
+  pl->mma = false;
+  const bool fp8 = p->kv_dtype == QMLA_DT_FP8E4M3;
+  const int es = fp8 ? 1 : 2;
+  TreeMma& m = pl->m;
+  memset(&m, 0, sizeof(m));
+  if (p->rank % 128 != 0 || p->rank > 768 || p->block_table_cols == 0 || p->num_reqs == 0 || p->num_nodes == 0) return;
+  m.run = gcd_int(p->page_size, 64);
+  m.chunks = (p->qk_dim * es + 127) / 128;
+  m.full_chunks = p->qk_dim * es / 128;
+  m.v_chunks = p->rank * es / 128;
+  m.terms = q_terms(fp8, p->q_dtype);
+  if (m.run < 16 || m.full_chunks < 2) return;
+  if (p->rms_mode != QMLA_RMS_NONE) {
+    const int bytes = p->num_heads * (!fp8 || p->rms_mode == QMLA_RMS_BF16 ? 2 : 1);
+    const int off = p->rms_offset * es;
+    m.base_b = off & ~15;
+    m.skip = off - m.base_b;
+    m.units = (m.skip + bytes + 15) / 16;
+    if (m.units > 7 || m.base_b + 16 * m.units > p->kv_row_width * es) return;
+  }
+  const int64_t rows = (int64_t)p->num_nodes * p->num_heads;
+  const int clusters = fp8 ? resident_clusters<true>(p->device) : resident_clusters<false>(p->device);
+  if (rows > (int64_t)128 * clusters) return;
+  m.rows = (int)rows;
+  m.groups = (int)((rows + 127) / 128);
+  m.ranges = std::min(clusters / m.groups, kMaxCtas);
+  const int64_t img = (int64_t)m.terms * m.chunks * kTrRows * 128;
+  const int64_t fac = (int64_t)p->num_heads * kTrFacPitch * 4;
+  const int64_t ring = std::min(di.max_smem, kMaxDynSmem) - 1024 - img - tr_p_bytes(fp8) - fac - 1024;
+  if (ring < 3 * (int64_t)kTrSlot) return;
+  m.nslots = (uint32_t)std::min<int64_t>(kTrMaxSlots, ring / kTrSlot);
+  m.img_bytes = (uint32_t)img;
+  m.off_q = m.nslots * kTrSlot;
+  m.off_p = m.off_q + (uint32_t)img;
+  m.off_fac = m.off_p + tr_p_bytes(fp8);
+  m.off_misc = m.off_fac + (uint32_t)fac;
+  pl->smem = m.off_misc + 1024 + 1024;
+  m.seg_cost = 2;
+  m.o_cols = fp8 ? (p->rank + 255) / 256 * 128 : p->rank / 2;
+  int64_t w = 0;
+  pl->ws_status = w;
+  w += 256;
+  pl->ws_prefix = w;
+  w = align_up(w + 4 * ((int64_t)p->num_reqs + 1), 256);
+  pl->ws_bounds = w;
+  w = align_up(w + 4 * ((int64_t)m.ranges + 1), 256);
+  pl->ws_img = w;
+  w = align_up(w + img * 2 * m.groups * p->num_reqs, 256);
+  pl->ws_qinv = w;
+  w = align_up(w + (int64_t)4 * 128 * m.groups * p->num_reqs, 256);
+  pl->ws_tail = w;
+  w = align_up(w + (int64_t)p->num_reqs * kTrTail * p->rank * es, 256);
+  pl->ws_lse = w;
+  w = align_up(w + (int64_t)2 * m.ranges * m.groups * 128 * 4, 256);
+  pl->ws_o = w;
+  w = align_up(w + (int64_t)2 * m.ranges * m.groups * 128 * 4 * p->rank, 256);
+  pl->ws_total = w;
+  pl->mma = true;
+}
 
 int make_tree_plan(const qmla_tree_params* p, TreePlan* pl) {
   if (!p || p->num_reqs < 0 || p->num_nodes < 0 || p->num_heads <= 0 || p->rank <= 0 || p->qk_dim < p->rank ||
@@ -306,6 +366,8 @@ int make_tree_plan(const qmla_tree_params* p, TreePlan* pl) {
   const int64_t rows = (int64_t)p->num_reqs * p->num_nodes;
   const int64_t blocks = rows * ((p->num_heads + kGenHeads - 1) / kGenHeads);
   if (blocks > INT32_MAX || rows * p->num_heads > INT32_MAX) return QMLA_E_UNSUPPORTED;
+  plan_mma(p, di, pl);
+  if (pl->mma) return QMLA_OK;
   // tokens split over blocks until every SM has two
   pl->nsplit = blocks == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(64, 2 * di.sms / blocks));
   int64_t w = 0;
@@ -330,6 +392,49 @@ int launch_generic(const TreeArgs& a, cudaStream_t st) {
   if (err != cudaSuccess) return QMLA_E_CUDA;
   const int hgroups = (a.heads + kGenHeads - 1) / kGenHeads;
   tree_generic_kernel<FP8><<<dim3(a.reqs * a.nodes * hgroups, a.nsplit), kGenThreads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+}
+
+template <bool FP8>
+int launch_tree_mma(const qmla_tree_params* p, const TreeArgs& a, const TreePlan& pl, uint8_t* ws, cudaStream_t st) {
+  const int es = FP8 ? 1 : 2;
+  TreeMma m = pl.m;
+  m.status = reinterpret_cast<int*>(ws + pl.ws_status);
+  m.prefix = reinterpret_cast<int32_t*>(ws + pl.ws_prefix);
+  m.bounds = reinterpret_cast<int32_t*>(ws + pl.ws_bounds);
+  m.img = ws + pl.ws_img;
+  m.q_inv = reinterpret_cast<float*>(ws + pl.ws_qinv);
+  m.tail = ws + pl.ws_tail;
+  m.part_lse = reinterpret_cast<float*>(ws + pl.ws_lse);
+  m.part_o = reinterpret_cast<float*>(ws + pl.ws_o);
+  const int osz = p->o_dtype == QMLA_DT_F32 ? 4 : 2;
+  m.o_vec = reinterpret_cast<uintptr_t>(p->o) % 16 == 0 && p->o_stride_row * osz % 16 == 0 && p->o_stride_head * osz % 16 == 0;
+  TreeMaps maps;
+  const cuuint64_t tok = p->kv_stride_token * es, page = p->kv_stride_page * es;
+  const cuuint32_t col = 128 / es;
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)p->qk_dim, (cuuint64_t)p->page_size, (cuuint64_t)p->kv_num_pages};
+    const cuuint64_t strides[2] = {tok, page};
+    const cuuint32_t box[3] = {col, (cuuint32_t)m.run, 1};
+    if (!encode_tiled(&maps.chunk, FP8, p->kv_cache, 3, dims, strides, box)) return QMLA_E_ALIGNMENT;
+  }
+  {
+    const cuuint64_t dims[5] = {col, 8, (cuuint64_t)m.full_chunks, (cuuint64_t)(p->page_size / 8), (cuuint64_t)p->kv_num_pages};
+    const cuuint64_t strides[4] = {tok, 128, 8 * tok, page};
+    const cuuint32_t box[5] = {col, 8, 2, (cuuint32_t)(m.run / 8), 1};
+    if (!encode_tiled(&maps.wide, FP8, p->kv_cache, 5, dims, strides, box)) return QMLA_E_ALIGNMENT;
+  }
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)p->rank, (cuuint64_t)p->num_reqs * kTrTail};
+    const cuuint64_t strides[1] = {(cuuint64_t)p->rank * es};
+    const cuuint32_t box[2] = {col, 64};
+    if (!encode_tiled(&maps.tail, FP8, m.tail, 2, dims, strides, box)) return QMLA_E_ALIGNMENT;
+  }
+  const int64_t warps = (int64_t)p->num_reqs * (m.groups * 128 + kTrTail);
+  if (warps / 8 + 1 > INT32_MAX) return QMLA_E_UNSUPPORTED;
+  tree_prep_kernel<FP8><<<(unsigned)((warps + 7) / 8 + 1), 256, 0, st>>>(a, m);
+  tree_mma_kernel<FP8><<<2 * m.ranges * m.groups, kTrThreads, pl.smem, st>>>(maps, a, m);
+  tree_pieces_kernel<<<dim3(p->num_reqs, m.rows), 128, 0, st>>>(a, m);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
 }
 
@@ -404,6 +509,7 @@ int qmla_tree_attention(const qmla_tree_params* p, void* stream) {
   a.part_lse = reinterpret_cast<float*>(ws + pl.ws_lse);
   a.part_o = reinterpret_cast<float*>(ws + pl.ws_o);
   a.nsplit = pl.nsplit;
+  if (pl.mma) return fp8 ? launch_tree_mma<true>(p, a, pl, ws, st) : launch_tree_mma<false>(p, a, pl, ws, st);
   rc = fp8 ? launch_generic<true>(a, st) : launch_generic<false>(a, st);
   if (rc != QMLA_OK) return rc;
   if (a.nsplit > 1) tree_join_kernel<<<a.reqs * a.nodes * a.heads, 128, 0, st>>>(a);

@@ -1,0 +1,845 @@
+// Tree attention on the tensor cores: two CTAs of a cluster work on 128 query rows of a request.
+//
+// The query rows of a request (node-major: row = node * heads + head) are cut into groups of 128; a
+// cluster walks a contiguous range of 128-token tiles for one group, 64 rows per CTA:
+//   S[128 rows, 128 tokens] = Q . K^T        tcgen05 cta_group::2, M = 128, K-major operands
+//   softmax per row, base 2, lazy rescale
+//   O[128 rows, rank]      += P . V          cta_group::2, M = 128, N = 256 dims, V MN-major
+// Why a pair.  32-bit accumulators of 768 output dims for 128 rows do not fit one SM's 512 TMEM
+// columns; of 64 rows they take 384 (a paired M = 128 tile keeps 64 rows per CTA, the first half of N
+// in lanes 0-63 and the second in lanes 64-127) and leave room for two S buffers.  And each CTA
+// supplies half of every B operand - K of 64 of the tile's tokens, V of half of the output dims - so
+// a byte brought into an SM serves 128 rows, not 64.  Q of 64 rows x 1000 dims takes 128 KB of shared
+// memory in either case; what is left streams K and V through one ring of 16 KB slots in the order
+// the MMAs take them: K(0), K(1), V(0), K(2), V(1), ... V is read again (from L2) because no SM can
+// hold a tile's keys until its softmax is done.
+// Groups of one request run side by side: cluster s * groups + g walks range s for group g, so
+// the groups' loads of a tile meet in L2 and the cache crosses HBM once.
+// A tile costs 63 + 24 MMAs, 3550 cycles at the dense rate whatever the rows in use (bf16; the
+// e4m3 form doubles the MMAs at twice the rate), against 224 KB into each SM: up to one group the call
+// is bound by HBM, beyond it by the tensor pipe and the L2-to-SM stream together.
+//
+// Weights P are rounded to bf16; over an FP8 cache to three e5m2 terms (at least 8 bits down to 2^-19 of
+// the row's largest weight, the last of them lost below 2^-29).  Two terms with an e4m3 one among them
+// are a third cheaper in PV but keep 3 bits or none below 2^-15, which a long faint tail behind one heavy
+// token cannot afford.
+// Values of drafted tokens and of the tail of the last page come from a copy with non-finite elements
+// zeroed (prep kernel): a node that does not see such a token has P = 0 there, and 0 * NaN must not
+// reach it; a node that sees it has S = NaN already.
+//
+// Warps of a CTA: 0-3 softmax and epilogue (a thread owns one row's 64 tokens), 4-7 score factors
+// (1 / rms per token and head, a token per thread), 8 TMA loads, 9 MMA issue (leader) or the
+// announcement that Q has landed (peer).
+#pragma once
+#include "qmla_decode.cuh"
+#include "qmla_pair.cuh"
+#include "qmla_qimage.cuh"
+
+namespace qmla {
+
+struct TreeArgs {
+  const uint8_t *q, *q_pe;
+  int64_t q_sr, q_sh, qpe_sr, qpe_sh;  // elements
+  int q_dtype;
+  const uint8_t* cache;
+  int64_t page_b, tok_b, num_pages;
+  const int32_t* bt;
+  int64_t bt_stride, bt_cols;
+  int page_size;
+  const int32_t* ctx;
+  const int64_t* mask;
+  int64_t mask_stride;  // elements between requests; 0: one tree for all
+  int reqs, nodes, heads, rank, qk_dim, rms_mode;
+  int64_t rms_off_b;
+  float sm_scale, logit_cap;
+  const float* k_scale;
+  uint8_t* o;
+  int64_t o_sr, o_sh;
+  int o_dtype;
+  uint8_t* lse;
+  int64_t lse_sr;
+  int lse_dtype;
+  float* part_o;    // [nsplit][rows][heads][rank]
+  float* part_lse;  // [nsplit][rows][heads], log2 units
+  int nsplit;
+};
+
+// Committed tokens of request r, clamped to what its block-table row can hold.
+__device__ __forceinline__ int tree_ctx(const TreeArgs& a, int r) {
+  const int64_t room = a.bt_cols * a.page_size;
+  return (int)min((int64_t)max(__ldg(a.ctx + r), 0), room);
+}
+
+constexpr int kTrThreads = 320;
+constexpr int kTrRows = 64;          // query rows per CTA
+constexpr int kTrTail = 256;         // tokens of a request's copied tail (127 + 64 at most)
+constexpr int kTrFacPitch = 132;     // floats between heads in the factor table
+constexpr int kTrMaxSlots = 10;
+constexpr uint32_t kTrSlot = 16384;
+constexpr int tr_p_bytes(bool fp8) { return fp8 ? 24576 : 16384; }  // P of a CTA's 64 rows x 128 tokens
+
+struct TreeMma {
+  int32_t* prefix;   // [reqs + 1] tiles
+  int32_t* bounds;   // [ranges + 1]
+  uint8_t* img;      // [reqs][groups][2][img_bytes]
+  float* q_inv;      // [reqs][groups][128] inverse query scalings (FP8)
+  uint8_t* tail;     // [reqs][kTrTail][rank]
+  float* part_o;     // [2 * ranges][groups][128][rank]
+  float* part_lse;   // [2 * ranges][groups][128], log2 units
+  int* status;
+  int groups, ranges, rows;  // rows = nodes * heads
+  int terms, chunks, full_chunks, v_chunks;
+  int run;                   // tokens per K / V box
+  int seg_cost;
+  uint32_t img_bytes, nslots, off_q, off_p, off_fac, off_misc;
+  int units, base_b, skip;   // rms tail: 16-byte units per token, first byte, bytes to skip
+  int o_cols;                // TMEM columns of O
+  int o_vec;                 // 16-byte stores of o are legal
+};
+struct TreeMaps {
+  CUtensorMap chunk;  // (element, token in page, page), box = one 128-byte column x run tokens
+  CUtensorMap wide;   // (element, token in group, column, group in page, page), box = 2 columns x run
+  CUtensorMap tail;   // (element, token), box = one 128-byte column x 64 tokens
+};
+
+// Tokens of request r: committed and drafted, within its block-table row.
+__device__ __forceinline__ int64_t tree_tokens(const TreeArgs& a, int r) {
+  return min((int64_t)tree_ctx(a, r) + a.nodes, a.bt_cols * a.page_size);
+}
+
+// Query images, the sanitised tail, the tile prefix and range bounds.  A warp per image row, then a
+// warp per tail token; the last block plans.
+template <bool FP8>
+__global__ void __launch_bounds__(256) tree_prep_kernel(const TreeArgs a, const TreeMma m) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t qrows = (int64_t)a.reqs * m.groups * 128, trows = (int64_t)a.reqs * kTrTail;
+  if (blockIdx.x + 1 < gridDim.x) {
+    int64_t w = (int64_t)blockIdx.x * 8 + warp;
+    if (w < qrows) {
+      const int r = (int)(w / (m.groups * 128)), x = (int)(w - (int64_t)r * m.groups * 128);
+      const int node = x / a.heads, h = x - node * a.heads;
+      const QSource s{a.q, a.q_pe, a.q_sr, a.q_sh, a.qpe_sr, a.qpe_sh, a.q_dtype, a.rank, a.qk_dim};
+      uint8_t* img = m.img + (w >> 6) * m.img_bytes;  // 64 rows per image
+      const float inv = write_q_row<FP8>(s, x < m.rows ? (int64_t)r * a.nodes + node : -1, h, img, x & 63, kTrRows,
+                                         m.chunks, m.terms);
+      if (lane == 0) m.q_inv[w] = inv;
+      return;
+    }
+    w -= qrows;
+    if (w >= trows) return;
+    const int r = (int)(w / kTrTail), i = (int)(w - (int64_t)r * kTrTail);
+    const int64_t n = tree_tokens(a, r), t = tree_ctx(a, r) / kTile * kTile + i;
+    if (t / kTile >= (n + kTile - 1) / kTile) return;  // no such tile
+    const uint8_t* src = nullptr;
+    if (t < n) {
+      const int pg = __ldg(a.bt + r * a.bt_stride + t / a.page_size);
+      if (pg >= 0 && pg < a.num_pages) src = a.cache + (int64_t)pg * a.page_b + t % a.page_size * a.tok_b;
+    }
+    const int units = a.rank * (FP8 ? 1 : 2) / 16;
+    uint4* dst = reinterpret_cast<uint4*>(m.tail + w * a.rank * (FP8 ? 1 : 2));
+    for (int u = lane; u < units; u += 32) {
+      uint4 v = src ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0u, 0u, 0u, 0u);
+      uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (FP8) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if ((e[k] >> (8 * b) & 0x7f) == 0x7f) e[k] &= ~(0xffu << (8 * b));
+        } else {
+          if ((e[k] & 0x7f80u) == 0x7f80u) e[k] &= 0xffff0000u;
+          if ((e[k] & 0x7f800000u) == 0x7f800000u) e[k] &= 0x0000ffffu;
+        }
+      }
+      dst[u] = v;
+    }
+    return;
+  }
+  __shared__ int warp_sum[8];
+  __shared__ int carry;
+  if (threadIdx.x == 0) {
+    carry = 0;
+    m.prefix[0] = 0;
+    *m.status = 0;
+  }
+  for (int base = 0; base < a.reqs; base += 256) {
+    const int i = base + threadIdx.x;
+    int x = i < a.reqs ? (int)((tree_tokens(a, i) + kTile - 1) / kTile) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    x += carry;
+    for (int w = 0; w < warp; ++w) x += warp_sum[w];
+    if (i < a.reqs) m.prefix[i + 1] = x;
+    __syncthreads();
+    if (threadIdx.x == 255) carry = x;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int c = threadIdx.x; c <= m.ranges; c += 256) m.bounds[c] = range_bound(m.prefix, a.reqs, m.ranges, m.seg_cost, c);
+}
+
+template <bool FP8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
+    tree_mma_kernel(const __grid_constant__ TreeMaps maps, const TreeArgs a, const TreeMma m) {
+  constexpr float kThr = FP8 ? 2.f : 8.f;    // log2 units a weight may exceed 1 by before O is rescaled
+  constexpr float kShift = FP8 ? 13.f : 0.f;  // P = 2^(x - m + shift), up to 2^15 where e5m2 ends
+  constexpr int kPTerms = FP8 ? 3 : 1;
+  constexpr int es = FP8 ? 1 : 2;
+  constexpr int E = 128 / es;                // elements of a 128-byte column
+  constexpr int NV = FP8 ? 1 : 2;            // token halves of a V tile held in slots of their own
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_rank();
+  const int cluster = blockIdx.x >> 1;
+  const int range = cluster / m.groups, g = cluster - range * m.groups;
+  const int lo = __ldg(m.bounds + range), hi = __ldg(m.bounds + range + 1);
+  if (lo >= hi) return;  // the same for both CTAs
+  const int req0 = first_row_at(m.prefix, a.reqs, lo);
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + m.off_misc);
+  // leader's: full (both CTAs' loads of a slot), sempty, pfull, ofree, qpeer.  Each CTA's own: empty,
+  // sfull, odone, qempty (all arrived on by the leader's commits), qfull, facfull, facfree.
+  const uint32_t b_full = 0, b_empty = m.nslots, b_sfull = 2 * m.nslots, b_sempty = b_sfull + 2, b_pfull = b_sempty + 2,
+                 b_odone = b_pfull + 1, b_ofree = b_odone + 1, b_qfull = b_ofree + 1, b_qempty = b_qfull + 1,
+                 b_qpeer = b_qempty + 1, b_facfull = b_qpeer + 1, b_facfree = b_facfull + 1, b_fin = b_facfree + 1,
+                 n_bars = b_fin + 1;
+  auto bar = [&](uint32_t i) { return smem_u32(bars + i); };
+  auto leader = [&](uint32_t i) { return map_cta(smem_u32(bars + i), 0); };
+  uint8_t* misc = reinterpret_cast<uint8_t*>(bars + n_bars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
+  volatile uint32_t* valid_s = reinterpret_cast<volatile uint32_t*>(misc + 16);  // [4] tokens that exist
+  float* red = reinterpret_cast<float*>(misc + 32);                              // [128]
+  float* fac = reinterpret_cast<float*>(smem + m.off_fac);                       // [heads][kTrFacPitch]
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < m.nslots; ++i) {
+      mbar_init(bar(b_full + i), 1);
+      mbar_init(bar(b_empty + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(b_sfull + i), 1);
+      mbar_init(bar(b_sempty + i), 8);
+    }
+    mbar_init(bar(b_pfull), 8);
+    mbar_init(bar(b_odone), 1);
+    mbar_init(bar(b_ofree), 8);
+    mbar_init(bar(b_qfull), 1);
+    mbar_init(bar(b_qempty), 1);
+    mbar_init(bar(b_qpeer), 1);
+    mbar_init(bar(b_facfull), 4);
+    mbar_init(bar(b_facfree), 4);
+    mbar_init(bar(b_fin), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are ready
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t col_s = m.o_cols;
+  const uint32_t qbuf = sbase + m.off_q, pbuf = sbase + m.off_p;
+  const int v_blocks = (m.v_chunks + 2 * NV - 1) / (2 * NV);  // 256-dim output blocks
+  // 128-byte V columns of block nb that CTA c holds: FP8 one (none past the rank), bf16 two, or
+  // one in a last block of 128 dims
+  auto v_cols = [&](int nb, int c) -> int {
+    if constexpr (FP8) return 2 * nb + c < m.v_chunks ? 1 : 0;
+    return m.v_chunks - 4 * nb >= 4 ? 2 : 1;
+  };
+  auto v_col0 = [&](int nb, int c) -> int { return FP8 ? 2 * nb + c : 4 * nb + c * v_cols(nb, c); };
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- loads
+    const uint64_t pol = policy_evict_normal();
+    const int run = m.run, khalf = 64 / run;  // boxes of a CTA's 64 tokens of K
+    const int k_slots = (m.chunks + 1) / 2;
+    const uint32_t full0 = leader(b_full);
+    SegCursor cur{req0, lo, hi};
+    int r, k0, k1, plo, phi;
+    uint32_t seg = 0, armed = 0;
+    Ring ring;
+    bool ok = true;
+    // the next slot: wait until it is free, arm the leader's barrier for both CTAs' bytes
+    auto slot_begin = [&](uint32_t bytes) -> bool {
+      bool good = true;
+      if (lane == 0) {
+        good = mbar_wait(bar(b_empty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
+        if (good && cta == 0) mbar_expect_tx(bar(b_full + ring.idx), bytes);
+      }
+      return __shfl_sync(0xffffffffu, good, 0);
+    };
+    while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+      if (lane == 0) {
+        if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
+        if (ok) {
+          mbar_expect_tx(bar(b_qfull), m.img_bytes);
+          load_image(qbuf, m.img + (((int64_t)r * m.groups + g) * 2 + cta) * m.img_bytes, m.img_bytes, bar(b_qfull), pol);
+          ++seg;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      const int64_t n = tree_tokens(a, r);
+      const int ctx = tree_ctx(a, r), tail_tile = ctx / kTile;
+      const int32_t* bt = a.bt + r * a.bt_stride;
+      auto run_page = [&](int k) -> int {  // page of token run `lane` of tile k, -1 past the end
+        const int64_t tok = (int64_t)k * kTile + lane * run;
+        return lane < 2 * khalf && tok < n ? __ldg(bt + tok / a.page_size) : -1;
+      };
+      int pg_prev = -1;
+      for (int k = k0; k <= k1 && ok; ++k) {
+        const int pg = k < k1 ? run_page(k) : -1;
+        if (k < k1) {  // K of tile k: this CTA's 64 tokens, two columns per slot
+          for (int s = 0; s < k_slots && ok; ++s) {
+            const int c0 = 2 * s, nch = min(2, m.chunks - c0);
+            ok = slot_begin((uint32_t)nch * 2u * 8192u);
+            if (!ok) break;
+            const uint32_t slot = sbase + ring.idx * kTrSlot, fb = full0 + ring.idx * 8;
+            const int b = lane % khalf, c = lane / khalf;
+            const int pgb = __shfl_sync(0xffffffffu, pg, (int)cta * khalf + b);
+            const int y = (int)(((int64_t)k * kTile + cta * 64 + b * run) % a.page_size);
+            if (c0 + 2 > m.full_chunks) {
+              if (c < nch) tma_load_3d_pair(slot + c * 8192 + b * run * 128, &maps.chunk, (c0 + c) * E, y, pgb, fb, pol);
+            } else if (lane < khalf) {
+              tma_load_5d_pair(slot + b * run * 256, &maps.wide, 0, 0, c0, y / 8, pgb, fb, pol);
+            }
+            ++armed;
+            ring.next(m.nslots);
+          }
+        }
+        if (k > k0) {  // V of tile k - 1: all its tokens, this CTA's half of the dims
+          const int kv = k - 1;
+          const bool tail = kv >= tail_tile;
+          const int row0 = r * kTrTail + (kv - tail_tile) * kTile;  // in the copied tail
+          for (int th = 0; th < NV && ok; ++th)
+            for (int nb = 0; nb < v_blocks && ok; ++nb) {
+              const int nc = v_cols(nb, (int)cta), vc0 = v_col0(nb, (int)cta);
+              const int toks = kTile / NV;
+              ok = slot_begin((uint32_t)((v_cols(nb, 0) + v_cols(nb, 1)) * toks * 128));
+              if (!ok) break;
+              const uint32_t slot = sbase + ring.idx * kTrSlot, fb = full0 + ring.idx * 8;
+              if (tail) {
+                const int nbox = nc * (toks / 64);
+                if (lane < nbox) {
+                  const int cc = NV == 2 ? lane : 0, tb = NV == 2 ? 0 : lane;
+                  tma_load_2d_pair(slot + lane * 8192, &maps.tail, (vc0 + cc) * E, row0 + th * 64 + tb * 64, fb, pol);
+                }
+              } else {
+                const int nbox = toks / run;
+                const int bi = th * khalf + lane % nbox;  // token run of the tile
+                const int pgb = __shfl_sync(0xffffffffu, pg_prev, bi);
+                const int y = (int)(((int64_t)kv * kTile + bi * run) % a.page_size);
+                if (lane < nbox && nc > 0) {
+                  if (nc == 2)
+                    tma_load_5d_pair(slot + lane * run * 256, &maps.wide, 0, 0, vc0, y / 8, pgb, fb, pol);
+                  else
+                    tma_load_3d_pair(slot + lane * run * 128, &maps.chunk, vc0 * E, y, pgb, fb, pol);
+                }
+              }
+              ++armed;
+              ring.next(m.nslots);
+            }
+        }
+        pg_prev = pg;
+      }
+    }
+    if (!ok && lane == 0) {  // after an abort: wait (bounded) for the copies already issued
+      volatile int never = 0;
+      if (cta == 0)
+        for (uint32_t p = armed > m.nslots ? armed - m.nslots : 0u; p < armed; ++p)
+          mbar_wait(bar(b_full + p % m.nslots), (p / m.nslots) & 1, &never, nullptr, 20000000ull);
+      if (seg > 0) mbar_wait(bar(b_qfull), (seg - 1) & 1, &never, nullptr, 20000000ull);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA issue
+    if (lane == 0) {
+      SegCursor cur{req0, lo, hi};
+      int r, k0, k1, plo, phi;
+      uint32_t seg = 0;
+      bool ok = true;
+      if (cta == 1) {  // tell the leader that this CTA's Q has landed
+        while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+          ok = mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status);
+          if (ok) mbar_arrive_cluster(leader(b_qpeer));
+          ++seg;
+        }
+      } else {
+        auto idesc = [](uint32_t fa, uint32_t fb, uint32_t N, uint32_t b_mn) {
+          return (1u << 4) | (fa << 7) | (fb << 10) | (b_mn << 16) | ((N >> 3) << 17) | ((128u >> 4) << 24);
+        };
+        const uint64_t q0 = make_sdesc(qbuf, 16, 1024, 2);
+        const uint32_t qt16 = (uint32_t)(m.chunks * kTrRows * 128) >> 4;
+        const uint64_t p0 = make_sdesc(pbuf, 16, 1024, 2);
+        const int k_slots = (m.chunks + 1) / 2;
+        uint32_t js = 0, jp = 0;  // tiles scored / accumulated so far
+        Ring ring;
+        auto qk = [&]() {
+          const uint32_t sb = js & 1;
+          if (js >= 2) ok = mbar_wait_cluster(bar(b_sempty + sb), ((js - 2) >> 1) & 1, abort_flag, m.status);
+          const uint32_t d = tmem + col_s + sb * 64;
+          for (int s = 0; s < k_slots && ok; ++s) {
+            ok = mbar_wait_cluster(bar(b_full + ring.idx), ring.ph, abort_flag, m.status);
+            if (!ok) return;
+            tc_fence_after();
+            const int c0 = 2 * s, nch = min(2, m.chunks - c0);
+            const bool plain = c0 + 2 > m.full_chunks;
+            const uint32_t slot = sbase + ring.idx * kTrSlot;
+            for (int ci = 0; ci < nch; ++ci) {
+              const uint64_t bd = plain ? make_sdesc(slot + ci * 8192, 16, 1024, 2) : make_sdesc(slot + ci * 1024, 16, 2048, 2);
+              for (int t = 0; t < m.terms; ++t) {
+                const uint64_t ad = q0 + (uint64_t)((c0 + ci) * (kTrRows * 128 >> 4)) + (uint64_t)t * qt16;
+                const uint32_t id_qk = FP8 ? idesc(q_term_format(t), 0, 128, 0) : idesc(1, 1, 128, 0);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                  const uint32_t acc = (s | ci | t | ks) != 0;
+                  if constexpr (FP8)
+                    tc_mma_f8_pair(d, ad + ks * 2, bd + ks * 2, id_qk, acc);
+                  else
+                    tc_mma_f16_pair(d, ad + ks * 2, bd + ks * 2, id_qk, acc);
+                }
+              }
+            }
+            tc_commit_pair(bar(b_empty + ring.idx));
+            ring.next(m.nslots);
+          }
+          if (ok) tc_commit_pair(bar(b_sfull + sb));
+          ++js;
+        };
+        while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+          ok = mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status) &&
+               mbar_wait_cluster(bar(b_qpeer), seg & 1, abort_flag, m.status);
+          if (!ok) break;
+          const int tail_tile = tree_ctx(a, r) / kTile;
+          qk();
+          for (int k = k0; k < k1 && ok; ++k) {
+            if (k + 1 < k1)
+              qk();
+            else
+              tc_commit_pair(bar(b_qempty));  // Q is free once the segment's scores are done
+            if (ok) ok = mbar_wait_cluster(bar(b_pfull), jp & 1, abort_flag, m.status);
+            if (ok && k == k0 && seg > 0) ok = mbar_wait_cluster(bar(b_ofree), (seg - 1) & 1, abort_flag, m.status);
+            const bool tail = k >= tail_tile;
+            for (int th = 0; th < NV && ok; ++th)
+              for (int nb = 0; nb < v_blocks && ok; ++nb) {
+                ok = mbar_wait_cluster(bar(b_full + ring.idx), ring.ph, abort_flag, m.status);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t slot = sbase + ring.idx * kTrSlot;
+                const uint32_t d = tmem + nb * 128;
+                if constexpr (FP8) {
+                  const uint64_t bd = make_sdesc(slot, 8192, 1024, 2);
+#pragma unroll
+                  for (int ks = 0; ks < 4; ++ks) {
+                    const uint32_t acc = k > k0 || ks > 0;
+#pragma unroll
+                    for (int t = 0; t < kPTerms; ++t)
+                      tc_mma_f8_pair(d, p0 + (uint64_t)(t * (8192 >> 4)) + ks * 2, bd + (uint64_t)(ks * (4096 >> 4)),
+                                     idesc(1, 0, 256, 1), acc || t > 0);
+                  }
+                } else {
+                  const int nc = v_cols(nb, 0);
+                  const uint32_t id = idesc(1, 1, nc == 2 ? 256 : 128, 1);
+                  // columns of the slot apart by LBO, 8-token groups by SBO
+                  const bool paired = nc == 2 && !tail;
+                  const uint64_t bd = paired ? make_sdesc(slot, 1024, 2048, 2) : make_sdesc(slot, 8192, 1024, 2);
+                  const uint32_t step = (paired ? 4096u : 2048u) >> 4;  // 16 tokens
+#pragma unroll
+                  for (int ks = 0; ks < 4; ++ks) {
+                    const uint32_t acc = k > k0 || th > 0 || ks > 0;
+                    tc_mma_f16_pair(d, p0 + (uint64_t)(th * (8192 >> 4)) + ks * 2, bd + (uint64_t)(ks * step), id, acc);
+                  }
+                }
+                tc_commit_pair(bar(b_empty + ring.idx));
+                ring.next(m.nslots);
+              }
+            if (ok) tc_commit_pair(bar(b_odone));
+            ++jp;
+          }
+          ++seg;
+        }
+        volatile int never = 0;  // drain before TMEM is released
+        tc_commit_pair(bar(b_fin));
+        mbar_wait(bar(b_fin), 0, &never, nullptr, 100000000ull);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- score factors, a token per thread
+    const int ft = threadIdx.x - 128;
+    const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
+    const float gs = a.sm_scale * kscale * (a.logit_cap > 0.f ? 1.f : kLog2e);
+    const int rb = !FP8 || a.rms_mode == 2 ? 2 : 1;  // bytes per divisor
+    SegCursor cur{req0, lo, hi};
+    int r, k0, k1, plo, phi;
+    uint32_t jt = 0;
+    bool ok = true;
+    while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+      const int64_t n = tree_tokens(a, r);
+      for (int k = k0; k < k1 && ok; ++k, ++jt) {
+        const int64_t t = (int64_t)k * kTile + ft;
+        alignas(16) uint8_t tailb[16 * 7];
+        bool here = false;
+        if (t < n) {
+          const int pg = __ldg(a.bt + r * a.bt_stride + t / a.page_size);
+          here = pg >= 0 && pg < a.num_pages;
+          if (here) {
+            const uint8_t* p = a.cache + (int64_t)pg * a.page_b + t % a.page_size * a.tok_b + m.base_b;
+            for (int u = 0; u < m.units; ++u) reinterpret_cast<uint4*>(tailb)[u] = __ldg(reinterpret_cast<const uint4*>(p) + u);
+          }
+        }
+        if (jt > 0) ok = mbar_wait(bar(b_facfree), (jt - 1) & 1, abort_flag, m.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        for (int h = 0; h < a.heads; ++h) {
+          float f = gs;
+          if (m.units > 0 && here) {
+            const uint8_t* b = tailb + m.skip + rb * h;
+            const uint32_t bits = rb == 1 ? *b : (uint32_t)b[0] | (uint32_t)b[1] << 8;
+            if (FP8 && a.rms_mode == 3) {
+              f *= ex2_approx(3.0f - (float)bits * (6.0f / 255.0f));
+            } else {
+              const float rv = (!FP8 || a.rms_mode == 2) ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits))
+                                                         : e4m3_to_f32((uint8_t)bits) * kscale;
+              f = rv > 0.f ? __fdividef(f, rv) : f;
+            }
+          }
+          fac[h * kTrFacPitch + ft] = f;
+        }
+        const unsigned v = __ballot_sync(0xffffffffu, here);
+        if (lane == 0) valid_s[warp - 4] = v;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(b_facfull));
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax and epilogue
+    const int l = threadIdx.x;              // TMEM lane
+    const int i = l & 63, half = l >> 6;    // row of the CTA; half of the tile's tokens, of a block's dims
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const int x_row = g * 128 + (int)cta * 64 + i;
+    const bool live = x_row < m.rows;
+    const int node = live ? x_row / a.heads : 0, h = live ? x_row - node * a.heads : 0;
+    const float* fac_row = fac + h * kTrFacPitch + half * 64;
+    const bool cap = a.logit_cap > 0.f;
+    const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
+    const uint32_t sempty0 = leader(b_sempty), pfull0 = leader(b_pfull), ofree0 = leader(b_ofree);
+    SegCursor cur{req0, lo, hi};
+    int r, k0, k1, plo, phi;
+    uint32_t jt = 0;
+    // ok: this warp's waits so far; dead: the four warps have agreed (in a group barrier) to leave
+    bool ok = true, dead = false;
+    while (!dead && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+      const int ctx = tree_ctx(a, r);
+      const uint64_t mask = live ? (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + r * a.mask_stride + node) &
+                                       (a.nodes >= 64 ? ~0ull : (1ull << a.nodes) - 1)
+                                 : 0ull;
+      const float q_inv = FP8 ? __ldg(m.q_inv + ((int64_t)r * m.groups + g) * 128 + cta * 64 + i) : 1.f;
+      float m_ref = -INFINITY, l_part = 0.f;
+      for (int k = k0; k < k1; ++k, ++jt) {
+        const uint32_t sb = jt & 1;
+        float x[64];
+        ok = ok && mbar_wait(bar(b_sfull + sb), (jt >> 1) & 1, abort_flag, m.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          tc_fence_after();
+          tmem_ld32(tmem + lane_base + col_s + sb * 64, x);
+          tmem_ld32(tmem + lane_base + col_s + sb * 64 + 32, x + 32);
+          tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(sempty0 + sb * 8);
+          ok = mbar_wait(bar(b_facfull), jt & 1, abort_flag, m.status);
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        uint64_t vis = 0;
+        if (ok) {
+#pragma unroll
+          for (int e = 0; e < 64; e += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(fac_row + e);
+            x[e] *= f.x;
+            x[e + 1] *= f.y;
+            x[e + 2] *= f.z;
+            x[e + 3] *= f.w;
+          }
+          vis = (uint64_t)valid_s[2 * half] | (uint64_t)valid_s[2 * half + 1] << 32;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(b_facfree));
+        }
+        if constexpr (FP8) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) x[e] *= q_inv;
+        }
+        if (cap) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) x[e] = a.logit_cap * tanhf(x[e] / a.logit_cap) * kLog2e;
+        }
+        // tokens this row sees: committed ones, and drafts of its mask
+        const int64_t b0 = (int64_t)k * kTile + half * 64;
+        if (b0 + 64 > ctx || mask == 0) {
+          const int64_t nc = (int64_t)ctx - b0;  // committed tokens of this half
+          uint64_t see = nc <= 0 ? 0ull : nc >= 64 ? ~0ull : (1ull << nc) - 1;
+          if (nc >= 0)
+            see |= nc < 64 ? mask << nc : 0ull;
+          else
+            see |= -nc < 64 ? mask >> -nc : 0ull;
+          vis &= mask == 0 ? 0ull : see;
+        }
+        float mx = -INFINITY;
+        if (vis == ~0ull) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) mx = fmaxf(mx, x[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            if (!(vis >> e & 1)) x[e] = -INFINITY;
+            mx = fmaxf(mx, x[e]);
+          }
+        }
+        bool need = mx > m_ref + kThr;
+        // one group barrier per tile reduces the rescale test and any failed wait
+        need = named_bar_or(1, 128, need || !ok);
+        if (need) {
+          dead = named_bar_or(1, 128, !ok);
+          if (dead) break;
+          red[l] = mx;
+          named_bar_sync(1, 128);
+          const float mn = fmaxf(m_ref, fmaxf(mx, red[l ^ 64]));
+          const float al = mn == m_ref ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - mn);
+          m_ref = mn;
+          l_part *= al;
+          if (named_bar_or(1, 128, al != 1.f && k > k0)) {  // (red[] is free again)
+            ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+              tc_fence_after();
+              for (int c = 0; c < m.o_cols; c += 16) {
+                float o[16];
+                tmem_ld16(tmem + lane_base + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= al;
+                tmem_st16(tmem + lane_base + c, o);
+              }
+              tmem_wait_st();
+              tc_fence_before();
+            }
+          }
+        }
+        // P = 2^(x - m): nothing where the row sees nothing (m = -inf)
+        const float sub = m_ref == -INFINITY && vis != ~0ull ? 0.f : m_ref - kShift;
+        uint32_t w[FP8 ? 48 : 32];
+        if constexpr (!FP8) {
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            const float pa = ex2_approx(x[e] - sub), pb = ex2_approx(x[e + 1] - sub);
+            l_part += pa + pb;
+            const __nv_bfloat162 b = __floats2bfloat162_rn(pa, pb);
+            w[e >> 1] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            w[q] = w[16 + q] = w[32 + q] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              float2 v = make_float2(ex2_approx(x[4 * q + e] - sub), ex2_approx(x[4 * q + e + 1] - sub));
+              l_part += v.x + v.y;
+#pragma unroll
+              for (int t = 0; t < kPTerms; ++t) {
+                const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E5M2);
+                w[16 * t + q] |= (uint32_t)b << (8 * e);
+                const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E5M2)));
+                v.x -= f.x;
+                v.y -= f.y;
+              }
+            }
+          }
+        }
+        // the P buffer is free, and O at rest, once the previous tile's PV is done
+        if (ok && jt > 0) ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          const uint32_t prow = pbuf + i * 128;
+          if constexpr (!FP8) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              st_shared_v4(prow + half * 8192 + ((u ^ (i & 7)) << 4), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const uint32_t at = prow + (((half * 4 + u) ^ (i & 7)) << 4);
+#pragma unroll
+              for (int t = 0; t < kPTerms; ++t)
+                st_shared_v4(at + t * 8192, w[16 * t + 4 * u], w[16 * t + 4 * u + 1], w[16 * t + 4 * u + 2], w[16 * t + 4 * u + 3]);
+            }
+          }
+          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(pfull0);
+        }
+      }
+      if (dead) break;
+      // ---- O / l -> the output, or this range's piece of it
+      ok = ok && mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
+      red[l] = l_part;
+      dead = named_bar_or(1, 128, !ok);
+      if (dead) break;
+      tc_fence_after();
+      const float lt = l_part + red[l ^ 64];
+      const float inv = lt == 0.f ? 0.f : kscale / lt;
+      const bool full = plo >= lo && phi <= hi;
+      const int64_t piece = ((int64_t)(plo <= lo ? 2 * range : 2 * range + 1) * m.groups + g) * 128 + cta * 64 + i;
+      const int64_t orow = (int64_t)r * a.nodes + node;
+      uint8_t* op = a.o + (orow * a.o_sr + (int64_t)h * a.o_sh) * dt_size(a.o_dtype);
+      for (int nb = 0; nb < v_blocks; ++nb) {
+        const int cols = FP8 ? 128 : 64 * v_cols(nb, 0);  // dims of this block in a lane
+        const int d0 = nb * 256 + half * cols;
+        for (int c = 0; c < cols; c += 16) {
+          float o[16];
+          tmem_ld16(tmem + lane_base + nb * 128 + c, o);
+          tmem_wait_ld();
+          if (!live || d0 + c >= a.rank) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = lt == 0.f ? 0.f : o[e] * inv;
+          if (!full) {
+            float4* p = reinterpret_cast<float4*>(m.part_o + piece * a.rank + d0 + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else if (a.o_dtype == 0 && m.o_vec) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
+              pk[e] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            uint4* p = reinterpret_cast<uint4*>(op + (int64_t)(d0 + c) * 2);
+            p[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            p[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              store_from_float(op + (int64_t)(d0 + c + e) * dt_size(a.o_dtype), a.o_dtype, o[e]);
+          }
+        }
+      }
+      if (live && half == 0) {
+        const float l2 = lt == 0.f ? -INFINITY : m_ref + log2f(lt) - kShift;
+        if (!full)
+          m.part_lse[piece] = l2;
+        else if (a.lse)
+          store_from_float(a.lse + (orow * a.lse_sr + h) * dt_size(a.lse_dtype), a.lse_dtype, l2 * kLn2);
+      }
+      tc_fence_before();
+      named_bar_sync(1, 128);  // red[] is read
+      if (lane == 0) mbar_arrive_cluster(ofree0);
+    }
+  }
+  // ---------------------------------------------------------------- teardown
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA leaves while the other may still signal it or read its tiles
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// Joins the pieces of requests cut at range boundaries: o = sum_i 2^(lse_i - lse) o_i.  One block per
+// (request, query row).  Requests inside one range are final already.
+__global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, const TreeMma m) {
+  const int r = blockIdx.x, x = blockIdx.y;
+  const int plo = __ldg(m.prefix + r), phi = __ldg(m.prefix + r + 1);
+  auto range_of = [&](int t) {  // the non-empty range that holds tile t
+    int lo = 0, hi = m.ranges;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(m.bounds + mid) <= t)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  if (phi == plo) return;
+  const int c0 = range_of(plo), c1 = range_of(phi - 1);
+  if (c0 == c1) return;
+  __shared__ float wts[kMaxCtas];
+  __shared__ int64_t at[kMaxCtas];
+  __shared__ int np_s;
+  __shared__ float inv_s;
+  const int g = x >> 7, i = x & 127;
+  if (threadIdx.x < 32) {
+    int np = 0;
+    for (int b = c0; b <= c1; b += 32) {
+      const int c = b + (int)threadIdx.x;
+      const bool in = c <= c1 && __ldg(m.bounds + c) < __ldg(m.bounds + c + 1);  // empty ranges wrote nothing
+      const unsigned bal = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        const int k = np + __popc(bal & ((1u << threadIdx.x) - 1));
+        const int slot = plo <= __ldg(m.bounds + c) ? 2 * c : 2 * c + 1;
+        at[k] = ((int64_t)slot * m.groups + g) * 128 + i;
+        wts[k] = __ldg(m.part_lse + at[k]);
+      }
+      np += __popc(bal);
+    }
+    __syncwarp();
+    float mx = -INFINITY;
+    bool bad = false;
+    for (int k = threadIdx.x; k < np; k += 32) {
+      mx = fmaxf(mx, wts[k]);
+      bad |= wts[k] != wts[k];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    bad = __any_sync(0xffffffffu, bad);
+    float sum = 0.f;
+    for (int k = threadIdx.x; k < np; k += 32) {
+      const float w = wts[k] == -INFINITY ? 0.f : exp2f(wts[k] - mx);
+      wts[k] = w;
+      sum += w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (bad) sum = NAN;
+    if (threadIdx.x == 0) {
+      np_s = np;
+      inv_s = sum == 0.f ? 0.f : 1.f / sum;
+      const int node = x / a.heads, h = x - node * a.heads;
+      if (a.lse)
+        store_from_float(a.lse + (((int64_t)r * a.nodes + node) * a.lse_sr + h) * dt_size(a.lse_dtype), a.lse_dtype,
+                         (mx + log2f(sum)) * kLn2);
+    }
+  }
+  __syncthreads();
+  const int np = np_s, node = x / a.heads, h = x - node * a.heads;
+  const float inv = inv_s;
+  uint8_t* op = a.o + (((int64_t)r * a.nodes + node) * a.o_sr + (int64_t)h * a.o_sh) * dt_size(a.o_dtype);
+  for (int d = threadIdx.x; d < a.rank; d += 128) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    int k = 0;
+    for (; k + 4 <= np; k += 4) {  // four loads in flight
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = __ldg(m.part_o + at[k + e] * a.rank + d);
+        acc[e] += wts[k + e] == 0.f ? 0.f : wts[k + e] * v;
+      }
+    }
+    for (; k < np; ++k) acc[0] += wts[k] == 0.f ? 0.f : wts[k] * __ldg(m.part_o + at[k] * a.rank + d);
+    store_from_float(op + (int64_t)d * dt_size(a.o_dtype), a.o_dtype, ((acc[0] + acc[1]) + (acc[2] + acc[3])) * inv);
+  }
+}
+
+}  // namespace qmla

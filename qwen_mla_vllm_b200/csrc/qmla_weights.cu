@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
   } else if (warp == 1) {
     // ---------------- S^T = K . Q^T
     if (lane == 0) {
-      const uint32_t idesc = make_idesc_f16(FP8 ? 0 : 1, 128, m.np, 0, 0);
+      // formats: bf16 both; or e4m3 keys and the term's format for Q
+      const uint32_t idesc0 = make_idesc_f16(FP8 ? 0 : 1, 128, m.np, 0, 0);
       const uint64_t q0 = make_sdesc(qbuf, 16, 1024, 2);
       const uint32_t qc16 = (uint32_t)m.np * 128 >> 4, qt16 = (uint32_t)(m.chunks * m.np) * 128 >> 4;
       SegCursor cur{req0, lo, hi};
@@ -344,6 +345,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                                         : make_sdesc(slot + ci * 1024, 16, 1024 * m.cps, 2);
               for (int t = 0; t < m.terms; ++t) {
                 const uint64_t bd = q0 + (uint64_t)(c0 + ci) * qc16 + (uint64_t)t * qt16;
+                const uint32_t idesc = idesc0 | (FP8 ? q_term_format(t) << 10 : 0u);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
                   const uint32_t acc = (s | ci | t | ks) != 0;
