@@ -35,30 +35,75 @@ struct QSource {
   int64_t q_sr, q_sh, qpe_sr, qpe_sh;  // elements
   int dtype;
   int rank, qk_dim;
+  int vec;  // rows may be read in 16-byte units (q_vec)
 };
 
-// Writes one row (all terms) of an image; src_row < 0 writes zeros.  One warp.  Returns the inverse
-// of the row's scaling in every lane.
+// Rows of q and q_pe start on 16-byte boundaries and hold whole 16-byte units.
+inline int q_vec(const void* q, int64_t sr, int64_t sh, const void* pe, int64_t psr, int64_t psh, int rank, int qk_dim) {
+  auto ok = [](const void* p, int64_t a, int64_t b) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 8 == 0 && b % 8 == 0;
+  };
+  return ok(q, sr, sh) && ok(pe, psr, psh) && rank % 8 == 0 && qk_dim % 8 == 0;
+}
+
+// Writes one row (all terms) of an image; src_row < 0 writes zeros.  One warp; a lane holds all its
+// units (of at most 2048 elements) before it converts any, so their loads overlap.  Returns the
+// inverse of the row's scaling in every lane.
 template <bool FP8>
 __device__ __forceinline__ float write_q_row(const QSource& s, int64_t src_row, int head, uint8_t* img, int row,
                                              int nrows, int chunks, int terms) {
-  constexpr int V = FP8 ? 16 : 8;  // elements of a 16-byte unit
+  constexpr int V = FP8 ? 16 : 8;        // elements of a 16-byte unit of the image
+  constexpr int U = 2048 / V / 32;       // units per lane at most
   const int lane = threadIdx.x & 31;
   const int units = chunks * 8;
   const int64_t term_bytes = (int64_t)chunks * nrows * 128;
-  auto elem = [&](int d) -> float {
-    if (src_row < 0 || d >= s.qk_dim) return 0.f;
-    return load_as_float(d < s.rank ? s.q + (src_row * s.q_sr + (int64_t)head * s.q_sh + d) * 2
-                                    : s.q_pe + (src_row * s.qpe_sr + (int64_t)head * s.qpe_sh + d - s.rank) * 2,
-                         s.dtype);
+  const uint8_t* q = s.q + (src_row * s.q_sr + (int64_t)head * s.q_sh) * 2;
+  const uint8_t* pe = s.q_pe + (src_row * s.qpe_sr + (int64_t)head * s.qpe_sh - s.rank) * 2;
+  uint4 raw[U][V / 8];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+#pragma unroll
+    for (int g = 0; g < V / 8; ++g) {
+      const int d = (lane + 32 * k) * V + 8 * g;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (src_row >= 0 && d < s.qk_dim) {
+        if (s.vec) {
+          v = __ldg(reinterpret_cast<const uint4*>((d < s.rank ? q : pe) + (int64_t)d * 2));
+        } else {
+          uint16_t e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            e[i] = d + i < s.qk_dim ? __ldg(reinterpret_cast<const uint16_t*>((d + i < s.rank ? q : pe) + (int64_t)(d + i) * 2)) : 0;
+          v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                         e[6] | (uint32_t)e[7] << 16);
+        }
+      }
+      raw[k][g] = v;
+    }
+  }
+  const bool bf = s.dtype == 0;
+  auto unpack = [&](const uint4& v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t lo = (uint16_t)w[i], hi = (uint16_t)(w[i] >> 16);
+      f[2 * i] = bf ? __bfloat162float(__ushort_as_bfloat16(lo)) : __half2float(__ushort_as_half(lo));
+      f[2 * i + 1] = bf ? __bfloat162float(__ushort_as_bfloat16(hi)) : __half2float(__ushort_as_half(hi));
+    }
   };
   float scale = 1.f;
   if constexpr (FP8) {
     float mx = 0.f;
-    for (int d = lane; d < s.qk_dim; d += 32) {
-      const float v = fabsf(elem(d));
-      if (v <= 3.0e38f) mx = fmaxf(mx, v);  // finite ones
-    }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int g = 0; g < V / 8; ++g) {
+        float f[8];
+        unpack(raw[k][g], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (fabsf(f[i]) <= 3.0e38f) mx = fmaxf(mx, fabsf(f[i]));  // finite ones
+      }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (mx > 0.f) {
@@ -67,16 +112,20 @@ __device__ __forceinline__ float write_q_row(const QSource& s, int64_t src_row, 
       if (mx * scale > 448.f) scale *= 0.5f;  // log2f may round up to a whole number
     }
   }
-  for (int u = lane; u < units; u += 32) {
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int u = lane + 32 * k;
+    if (u >= units) break;
     float v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = elem(u * V + e) * scale;
+    for (int g = 0; g < V / 8; ++g) unpack(raw[k][g], v + 8 * g);
     const int64_t at = (int64_t)(u >> 3) * nrows * 128 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
     for (int t = 0; t < terms; ++t) {
       uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         if constexpr (FP8) {
+          if (t == 0) v[e] *= scale;
           const bool fin = fabsf(v[e]) <= 448.f;  // not finite: NaN
           const uint8_t b = !fin ? 0x7f : t == 0 ? f32_to_e4m3(v[e]) : f32_to_e5m2(v[e]);
           w[e >> 2] |= (uint32_t)b << (8 * (e & 3));

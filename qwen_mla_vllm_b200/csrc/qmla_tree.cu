@@ -310,7 +310,7 @@ void plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
   m.ranges = std::min(clusters / m.groups, kMaxCtas);
   const int64_t img = (int64_t)m.terms * m.chunks * kTrRows * 128;
   const int64_t fac = (int64_t)p->num_heads * kTrFacPitch * 4;
-  const int64_t ring = std::min(di.max_smem, kMaxDynSmem) - 1024 - img - tr_p_bytes(fp8) - fac - 1024;
+  const int64_t ring = std::min(di.max_smem, kMaxDynSmem) - 1024 - img - tr_p_bytes(fp8) - fac - 2048;
   if (ring < 3 * (int64_t)kTrSlot) return;
   m.nslots = (uint32_t)std::min<int64_t>(kTrMaxSlots, ring / kTrSlot);
   m.img_bytes = (uint32_t)img;
@@ -318,7 +318,7 @@ void plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
   m.off_p = m.off_q + (uint32_t)img;
   m.off_fac = m.off_p + tr_p_bytes(fp8);
   m.off_misc = m.off_fac + (uint32_t)fac;
-  pl->smem = m.off_misc + 1024 + 1024;
+  pl->smem = m.off_misc + 2048 + 1024;
   m.seg_cost = 2;
   m.o_cols = fp8 ? (p->rank + 255) / 256 * 128 : p->rank / 2;
   int64_t w = 0;
@@ -409,6 +409,7 @@ int launch_tree_mma(const qmla_tree_params* p, const TreeArgs& a, const TreePlan
   m.part_o = reinterpret_cast<float*>(ws + pl.ws_o);
   const int osz = p->o_dtype == QMLA_DT_F32 ? 4 : 2;
   m.o_vec = reinterpret_cast<uintptr_t>(p->o) % 16 == 0 && p->o_stride_row * osz % 16 == 0 && p->o_stride_head * osz % 16 == 0;
+  m.q_vec = q_vec(a.q, a.q_sr, a.q_sh, a.q_pe, a.qpe_sr, a.qpe_sh, a.rank, a.qk_dim);
   TreeMaps maps;
   const cuuint64_t tok = p->kv_stride_token * es, page = p->kv_stride_page * es;
   const cuuint32_t col = 128 / es;

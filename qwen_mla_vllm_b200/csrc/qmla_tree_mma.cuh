@@ -27,8 +27,8 @@
 // zeroed (prep kernel): a node that does not see such a token has P = 0 there, and 0 * NaN must not
 // reach it; a node that sees it has S = NaN already.
 //
-// Warps of a CTA: 0-3 softmax and epilogue (a thread owns one row's 64 tokens), 4-7 score factors
-// (1 / rms per token and head, a token per thread), 8 TMA loads, 9 MMA issue (leader) or the
+// Warps of a CTA: 0-7 softmax and epilogue (a thread owns 32 tokens of one row), 8-11 score factors
+// (1 / rms per token and head, a token per thread), 12 TMA loads, 13 MMA issue (leader) or the
 // announcement that Q has landed (peer).
 #pragma once
 #include "qmla_decode.cuh"
@@ -70,7 +70,9 @@ __device__ __forceinline__ int tree_ctx(const TreeArgs& a, int r) {
   return (int)min((int64_t)max(__ldg(a.ctx + r), 0), room);
 }
 
-constexpr int kTrThreads = 320;
+constexpr int kTrSoftWarps = 8, kTrFacWarp = 8, kTrLoadWarp = 12, kTrMmaWarp = 13;
+constexpr int kTrThreads = 448;
+constexpr int kTrSoft = 32 * kTrSoftWarps;  // softmax threads
 constexpr int kTrRows = 64;          // query rows per CTA
 constexpr int kTrTail = 256;         // tokens of a request's copied tail (127 + 64 at most)
 constexpr int kTrFacPitch = 132;     // floats between heads in the factor table
@@ -94,7 +96,7 @@ struct TreeMma {
   uint32_t img_bytes, nslots, off_q, off_p, off_fac, off_misc;
   int units, base_b, skip;   // rms tail: 16-byte units per token, first byte, bytes to skip
   int o_cols;                // TMEM columns of O
-  int o_vec;                 // 16-byte stores of o are legal
+  int o_vec, q_vec;          // 16-byte accesses of o / q are legal
 };
 struct TreeMaps {
   CUtensorMap chunk;  // (element, token in page, page), box = one 128-byte column x run tokens
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const TreeArgs a, const 
     if (w < qrows) {
       const int r = (int)(w / (m.groups * 128)), x = (int)(w - (int64_t)r * m.groups * 128);
       const int node = x / a.heads, h = x - node * a.heads;
-      const QSource s{a.q, a.q_pe, a.q_sr, a.q_sh, a.qpe_sr, a.qpe_sh, a.q_dtype, a.rank, a.qk_dim};
+      const QSource s{a.q, a.q_pe, a.q_sr, a.q_sh, a.qpe_sr, a.qpe_sh, a.q_dtype, a.rank, a.qk_dim, m.q_vec};
       uint8_t* img = m.img + (w >> 6) * m.img_bytes;  // 64 rows per image
       const float inv = write_q_row<FP8>(s, x < m.rows ? (int64_t)r * a.nodes + node : -1, h, img, x & 63, kTrRows,
                                          m.chunks, m.terms);
@@ -217,7 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
   volatile uint32_t* valid_s = reinterpret_cast<volatile uint32_t*>(misc + 16);  // [4] tokens that exist
-  float* red = reinterpret_cast<float*>(misc + 32);                              // [128]
+  float* red = reinterpret_cast<float*>(misc + 32);                              // [4][64]
   float* fac = reinterpret_cast<float*>(smem + m.off_fac);                       // [heads][kTrFacPitch]
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < m.nslots; ++i) {
@@ -226,21 +228,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(b_sfull + i), 1);
-      mbar_init(bar(b_sempty + i), 8);
+      mbar_init(bar(b_sempty + i), 2 * kTrSoftWarps);
     }
-    mbar_init(bar(b_pfull), 8);
+    mbar_init(bar(b_pfull), 2 * kTrSoftWarps);
     mbar_init(bar(b_odone), 1);
-    mbar_init(bar(b_ofree), 8);
+    mbar_init(bar(b_ofree), 2 * kTrSoftWarps);
     mbar_init(bar(b_qfull), 1);
     mbar_init(bar(b_qempty), 1);
     mbar_init(bar(b_qpeer), 1);
     mbar_init(bar(b_facfull), 4);
-    mbar_init(bar(b_facfree), 4);
+    mbar_init(bar(b_facfree), kTrSoftWarps);
     mbar_init(bar(b_fin), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kTrMmaWarp) {
     tmem_alloc_pair(smem_u32(tmem_slot), 512);
     tmem_relinquish_pair();
   }
@@ -248,7 +250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers are ready
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t col_s = m.o_cols;
   const uint32_t qbuf = sbase + m.off_q, pbuf = sbase + m.off_p;
   const int v_blocks = (m.v_chunks + 2 * NV - 1) / (2 * NV);  // 256-dim output blocks
@@ -260,98 +262,102 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
   };
   auto v_col0 = [&](int nb, int c) -> int { return FP8 ? 2 * nb + c : 4 * nb + c * v_cols(nb, c); };
 
-  if (warp == 8) {
+  if (warp == kTrLoadWarp) {
     // ---------------------------------------------------------------- loads
+    // All lanes wait for a slot; lane 0 arms the leader's barrier for both CTAs' bytes; each of the
+    // first lanes issues one box.  What a box needs beside its column is worked out once per tile.
     const uint64_t pol = policy_evict_normal();
     const int run = m.run, khalf = 64 / run;  // boxes of a CTA's 64 tokens of K
     const int k_slots = (m.chunks + 1) / 2;
     const uint32_t full0 = leader(b_full);
+    const int kb = lane % khalf, kc = lane / khalf;        // this lane's K box: run, column (plain slots)
+    const int vbox = (kTile / NV) / run, vb = lane % vbox;  // V boxes of a slot, this lane's
+    const uint32_t k_wide = kb * run * 256, k_plain = kc * 8192 + kb * run * 128;
     SegCursor cur{req0, lo, hi};
     int r, k0, k1, plo, phi;
     uint32_t seg = 0, armed = 0;
     Ring ring;
     bool ok = true;
-    // the next slot: wait until it is free, arm the leader's barrier for both CTAs' bytes
-    auto slot_begin = [&](uint32_t bytes) -> bool {
-      bool good = true;
-      if (lane == 0) {
-        good = mbar_wait(bar(b_empty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
-        if (good && cta == 0) mbar_expect_tx(bar(b_full + ring.idx), bytes);
-      }
-      return __shfl_sync(0xffffffffu, good, 0);
+    auto slot_begin = [&](uint32_t bytes) {
+      ok = mbar_wait(bar(b_empty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && cta == 0 && lane == 0) mbar_expect_tx(bar(b_full + ring.idx), bytes);
     };
     while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+      if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       if (lane == 0) {
-        if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
-        if (ok) {
-          mbar_expect_tx(bar(b_qfull), m.img_bytes);
-          load_image(qbuf, m.img + (((int64_t)r * m.groups + g) * 2 + cta) * m.img_bytes, m.img_bytes, bar(b_qfull), pol);
-          ++seg;
-        }
+        mbar_expect_tx(bar(b_qfull), m.img_bytes);
+        load_image(qbuf, m.img + (((int64_t)r * m.groups + g) * 2 + cta) * m.img_bytes, m.img_bytes, bar(b_qfull), pol);
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      const int64_t n = tree_tokens(a, r);
-      const int ctx = tree_ctx(a, r), tail_tile = ctx / kTile;
+      ++seg;
+      const int n = (int)tree_tokens(a, r);
+      const int tail_tile = tree_ctx(a, r) / kTile;
       const int32_t* bt = a.bt + r * a.bt_stride;
-      auto run_page = [&](int k) -> int {  // page of token run `lane` of tile k, -1 past the end
-        const int64_t tok = (int64_t)k * kTile + lane * run;
-        return lane < 2 * khalf && tok < n ? __ldg(bt + tok / a.page_size) : -1;
+      int pg_next = -1, y_next = 0;  // page (-1 past the end) and row in it of token run `lane` of a tile
+      auto look_up = [&](int k) {
+        const uint32_t tok = (uint32_t)k * kTile + lane * run;
+        pg_next = -1;
+        if (lane < 2 * khalf && tok < (uint32_t)n) {
+          const uint32_t pi = tok / (uint32_t)a.page_size;
+          y_next = (int)(tok - pi * (uint32_t)a.page_size);
+          pg_next = __ldg(bt + pi);
+        }
       };
-      int pg_prev = -1;
+      look_up(k0);
+      int pg_prev = -1, y_prev = 0;
       for (int k = k0; k <= k1 && ok; ++k) {
-        const int pg = k < k1 ? run_page(k) : -1;
+        const int pg = pg_next, y = y_next;
+        if (k + 1 < k1) look_up(k + 1);  // on its way during this tile
         if (k < k1) {  // K of tile k: this CTA's 64 tokens, two columns per slot
-          for (int s = 0; s < k_slots && ok; ++s) {
+          const int kpg = __shfl_sync(0xffffffffu, pg, (int)cta * khalf + kb);
+          const int ky = __shfl_sync(0xffffffffu, y, (int)cta * khalf + kb);
+          for (int s = 0; s < k_slots; ++s) {
             const int c0 = 2 * s, nch = min(2, m.chunks - c0);
-            ok = slot_begin((uint32_t)nch * 2u * 8192u);
+            slot_begin((uint32_t)nch * 2u * 8192u);
             if (!ok) break;
             const uint32_t slot = sbase + ring.idx * kTrSlot, fb = full0 + ring.idx * 8;
-            const int b = lane % khalf, c = lane / khalf;
-            const int pgb = __shfl_sync(0xffffffffu, pg, (int)cta * khalf + b);
-            const int y = (int)(((int64_t)k * kTile + cta * 64 + b * run) % a.page_size);
             if (c0 + 2 > m.full_chunks) {
-              if (c < nch) tma_load_3d_pair(slot + c * 8192 + b * run * 128, &maps.chunk, (c0 + c) * E, y, pgb, fb, pol);
+              if (kc < nch) tma_load_3d_pair(slot + k_plain, &maps.chunk, (c0 + kc) * E, ky, kpg, fb, pol);
             } else if (lane < khalf) {
-              tma_load_5d_pair(slot + b * run * 256, &maps.wide, 0, 0, c0, y / 8, pgb, fb, pol);
+              tma_load_5d_pair(slot + k_wide, &maps.wide, 0, 0, c0, ky >> 3, kpg, fb, pol);
             }
             ++armed;
             ring.next(m.nslots);
           }
         }
-        if (k > k0) {  // V of tile k - 1: all its tokens, this CTA's half of the dims
+        if (k > k0 && ok) {  // V of tile k - 1: all its tokens, this CTA's half of the dims
           const int kv = k - 1;
           const bool tail = kv >= tail_tile;
           const int row0 = r * kTrTail + (kv - tail_tile) * kTile;  // in the copied tail
-          for (int th = 0; th < NV && ok; ++th)
-            for (int nb = 0; nb < v_blocks && ok; ++nb) {
+          for (int th = 0; th < NV && ok; ++th) {
+            const int vpg = __shfl_sync(0xffffffffu, pg_prev, th * khalf + vb);
+            const int vy = __shfl_sync(0xffffffffu, y_prev, th * khalf + vb);
+            for (int nb = 0; nb < v_blocks; ++nb) {
               const int nc = v_cols(nb, (int)cta), vc0 = v_col0(nb, (int)cta);
-              const int toks = kTile / NV;
-              ok = slot_begin((uint32_t)((v_cols(nb, 0) + v_cols(nb, 1)) * toks * 128));
+              constexpr int toks = kTile / NV;
+              slot_begin((uint32_t)((v_cols(nb, 0) + v_cols(nb, 1)) * toks * 128));
               if (!ok) break;
               const uint32_t slot = sbase + ring.idx * kTrSlot, fb = full0 + ring.idx * 8;
               if (tail) {
-                const int nbox = nc * (toks / 64);
-                if (lane < nbox) {
+                if (lane < nc * (toks / 64)) {
                   const int cc = NV == 2 ? lane : 0, tb = NV == 2 ? 0 : lane;
                   tma_load_2d_pair(slot + lane * 8192, &maps.tail, (vc0 + cc) * E, row0 + th * 64 + tb * 64, fb, pol);
                 }
-              } else {
-                const int nbox = toks / run;
-                const int bi = th * khalf + lane % nbox;  // token run of the tile
-                const int pgb = __shfl_sync(0xffffffffu, pg_prev, bi);
-                const int y = (int)(((int64_t)kv * kTile + bi * run) % a.page_size);
-                if (lane < nbox && nc > 0) {
-                  if (nc == 2)
-                    tma_load_5d_pair(slot + lane * run * 256, &maps.wide, 0, 0, vc0, y / 8, pgb, fb, pol);
-                  else
-                    tma_load_3d_pair(slot + lane * run * 128, &maps.chunk, vc0 * E, y, pgb, fb, pol);
-                }
+              } else if (lane < vbox && nc > 0) {
+                if (nc == 2)
+                  tma_load_5d_pair(slot + lane * run * 256, &maps.wide, 0, 0, vc0, vy >> 3, vpg, fb, pol);
+                else
+                  tma_load_3d_pair(slot + lane * run * 128, &maps.chunk, vc0 * E, vy, vpg, fb, pol);
               }
               ++armed;
               ring.next(m.nslots);
             }
+          }
         }
         pg_prev = pg;
+        y_prev = y;
       }
     }
     if (!ok && lane == 0) {  // after an abort: wait (bounded) for the copies already issued
@@ -362,122 +368,121 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       if (seg > 0) mbar_wait(bar(b_qfull), (seg - 1) & 1, &never, nullptr, 20000000ull);
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kTrMmaWarp) {
     // ---------------------------------------------------------------- MMA issue
-    if (lane == 0) {
-      SegCursor cur{req0, lo, hi};
-      int r, k0, k1, plo, phi;
-      uint32_t seg = 0;
-      bool ok = true;
-      if (cta == 1) {  // tell the leader that this CTA's Q has landed
-        while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-          ok = mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status);
-          if (ok) mbar_arrive_cluster(leader(b_qpeer));
-          ++seg;
-        }
-      } else {
-        auto idesc = [](uint32_t fa, uint32_t fb, uint32_t N, uint32_t b_mn) {
-          return (1u << 4) | (fa << 7) | (fb << 10) | (b_mn << 16) | ((N >> 3) << 17) | ((128u >> 4) << 24);
-        };
-        const uint64_t q0 = make_sdesc(qbuf, 16, 1024, 2);
-        const uint32_t qt16 = (uint32_t)(m.chunks * kTrRows * 128) >> 4;
-        const uint64_t p0 = make_sdesc(pbuf, 16, 1024, 2);
-        const int k_slots = (m.chunks + 1) / 2;
-        uint32_t js = 0, jp = 0;  // tiles scored / accumulated so far
-        Ring ring;
-        auto qk = [&]() {
-          const uint32_t sb = js & 1;
-          if (js >= 2) ok = mbar_wait_cluster(bar(b_sempty + sb), ((js - 2) >> 1) & 1, abort_flag, m.status);
-          const uint32_t d = tmem + col_s + sb * 64;
-          for (int s = 0; s < k_slots && ok; ++s) {
-            ok = mbar_wait_cluster(bar(b_full + ring.idx), ring.ph, abort_flag, m.status);
-            if (!ok) return;
-            tc_fence_after();
-            const int c0 = 2 * s, nch = min(2, m.chunks - c0);
-            const bool plain = c0 + 2 > m.full_chunks;
-            const uint32_t slot = sbase + ring.idx * kTrSlot;
-            for (int ci = 0; ci < nch; ++ci) {
-              const uint64_t bd = plain ? make_sdesc(slot + ci * 8192, 16, 1024, 2) : make_sdesc(slot + ci * 1024, 16, 2048, 2);
-              for (int t = 0; t < m.terms; ++t) {
-                const uint64_t ad = q0 + (uint64_t)((c0 + ci) * (kTrRows * 128 >> 4)) + (uint64_t)t * qt16;
-                const uint32_t id_qk = FP8 ? idesc(q_term_format(t), 0, 128, 0) : idesc(1, 1, 128, 0);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                  const uint32_t acc = (s | ci | t | ks) != 0;
-                  if constexpr (FP8)
-                    tc_mma_f8_pair(d, ad + ks * 2, bd + ks * 2, id_qk, acc);
-                  else
-                    tc_mma_f16_pair(d, ad + ks * 2, bd + ks * 2, id_qk, acc);
-                }
-              }
-            }
-            tc_commit_pair(bar(b_empty + ring.idx));
-            ring.next(m.nslots);
-          }
-          if (ok) tc_commit_pair(bar(b_sfull + sb));
-          ++js;
-        };
-        while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-          ok = mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status) &&
-               mbar_wait_cluster(bar(b_qpeer), seg & 1, abort_flag, m.status);
-          if (!ok) break;
-          const int tail_tile = tree_ctx(a, r) / kTile;
-          qk();
-          for (int k = k0; k < k1 && ok; ++k) {
-            if (k + 1 < k1)
-              qk();
-            else
-              tc_commit_pair(bar(b_qempty));  // Q is free once the segment's scores are done
-            if (ok) ok = mbar_wait_cluster(bar(b_pfull), jp & 1, abort_flag, m.status);
-            if (ok && k == k0 && seg > 0) ok = mbar_wait_cluster(bar(b_ofree), (seg - 1) & 1, abort_flag, m.status);
-            const bool tail = k >= tail_tile;
-            for (int th = 0; th < NV && ok; ++th)
-              for (int nb = 0; nb < v_blocks && ok; ++nb) {
-                ok = mbar_wait_cluster(bar(b_full + ring.idx), ring.ph, abort_flag, m.status);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t slot = sbase + ring.idx * kTrSlot;
-                const uint32_t d = tmem + nb * 128;
-                if constexpr (FP8) {
-                  const uint64_t bd = make_sdesc(slot, 8192, 1024, 2);
-#pragma unroll
-                  for (int ks = 0; ks < 4; ++ks) {
-                    const uint32_t acc = k > k0 || ks > 0;
-#pragma unroll
-                    for (int t = 0; t < kPTerms; ++t)
-                      tc_mma_f8_pair(d, p0 + (uint64_t)(t * (8192 >> 4)) + ks * 2, bd + (uint64_t)(ks * (4096 >> 4)),
-                                     idesc(1, 0, 256, 1), acc || t > 0);
-                  }
-                } else {
-                  const int nc = v_cols(nb, 0);
-                  const uint32_t id = idesc(1, 1, nc == 2 ? 256 : 128, 1);
-                  // columns of the slot apart by LBO, 8-token groups by SBO
-                  const bool paired = nc == 2 && !tail;
-                  const uint64_t bd = paired ? make_sdesc(slot, 1024, 2048, 2) : make_sdesc(slot, 8192, 1024, 2);
-                  const uint32_t step = (paired ? 4096u : 2048u) >> 4;  // 16 tokens
-#pragma unroll
-                  for (int ks = 0; ks < 4; ++ks) {
-                    const uint32_t acc = k > k0 || th > 0 || ks > 0;
-                    tc_mma_f16_pair(d, p0 + (uint64_t)(th * (8192 >> 4)) + ks * 2, bd + (uint64_t)(ks * step), id, acc);
-                  }
-                }
-                tc_commit_pair(bar(b_empty + ring.idx));
-                ring.next(m.nslots);
-              }
-            if (ok) tc_commit_pair(bar(b_odone));
-            ++jp;
-          }
-          ++seg;
-        }
-        volatile int never = 0;  // drain before TMEM is released
-        tc_commit_pair(bar(b_fin));
-        mbar_wait(bar(b_fin), 0, &never, nullptr, 100000000ull);
+    SegCursor cur{req0, lo, hi};
+    int r, k0, k1, plo, phi;
+    uint32_t seg = 0;
+    bool ok = true;
+    if (cta == 1) {  // tell the leader that this CTA's Q has landed
+      while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status));
+        if (ok && lane == 0) mbar_arrive_cluster(leader(b_qpeer));
+        ++seg;
       }
+    } else {
+      auto idesc = [](uint32_t fa, uint32_t fb, uint32_t N, uint32_t b_mn) {
+        return (1u << 4) | (fa << 7) | (fb << 10) | (b_mn << 16) | ((N >> 3) << 17) | ((128u >> 4) << 24);
+      };
+      const uint32_t q_lo = sdesc_lo(qbuf, 16), p_lo = sdesc_lo(pbuf, 16);
+      const uint32_t qt16 = (uint32_t)(m.chunks * kTrRows * 128) >> 4;
+      const uint32_t slot0 = sbase >> 4;
+      const int k_slots = (m.chunks + 1) / 2;
+      uint32_t js = 0, jp = 0;  // tiles scored / accumulated so far
+      Ring ring;
+      auto wait = [&](uint32_t b, uint32_t ph) {  // the whole warp
+        ok = ok && mbar_wait_cluster(bar(b), ph, abort_flag, m.status);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      auto qk = [&]() {
+        const uint32_t sb = js & 1;
+        if (js >= 2) wait(b_sempty + sb, ((js - 2) >> 1) & 1);
+        const uint32_t d = tmem + col_s + sb * 64;
+        for (int s = 0; s < k_slots; ++s) {
+          wait(b_full + ring.idx, ring.ph);
+          if (!ok) return;
+          tc_fence_after();
+          const bool plain = 2 * s + 2 > m.full_chunks;
+          const bool two = 2 * s + 1 < m.chunks;
+          // column ci of the slot: 8 KB on, or between the 8-row groups
+          const uint32_t b_lo = slot0 + ring.idx * (kTrSlot >> 4) + (1u << 16), b_hi = plain ? sdesc_hi(1024) : sdesc_hi(2048);
+          const uint32_t b_col = plain ? 8192 >> 4 : 1024 >> 4;
+          const uint32_t a_lo = q_lo + (uint32_t)s * (2 * kTrRows * 128 >> 4);
+#pragma unroll
+          for (int ci = 0; ci < 2; ++ci) {
+            if (ci == 1 && !two) break;
+            for (int t = 0; t < m.terms; ++t) {
+              const uint32_t id = FP8 ? idesc(q_term_format(t), 0, 128, 0) : idesc(1, 1, 128, 0);
+              const uint32_t al = a_lo + ci * (kTrRows * 128 >> 4) + t * qt16, bl = b_lo + ci * b_col;
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma_pair<FP8>(d, al + ks * 2, sdesc_hi(1024), bl + ks * 2, b_hi, id, (s | ci | t | ks) != 0);
+            }
+          }
+          tc_commit_pair(bar(b_empty + ring.idx));
+          ring.next(m.nslots);
+        }
+        tc_commit_pair(bar(b_sfull + sb));
+        ++js;
+      };
+      while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+        wait(b_qfull, seg & 1);
+        wait(b_qpeer, seg & 1);
+        if (!ok) break;
+        const int tail_tile = tree_ctx(a, r) / kTile;
+        qk();
+        for (int k = k0; k < k1 && ok; ++k) {
+          if (k + 1 < k1)
+            qk();
+          else
+            tc_commit_pair(bar(b_qempty));  // Q is free once the segment's scores are done
+          wait(b_pfull, jp & 1);
+          if (k == k0 && seg > 0) wait(b_ofree, (seg - 1) & 1);
+          const bool tail = k >= tail_tile;
+          for (int th = 0; th < NV && ok; ++th)
+            for (int nb = 0; nb < v_blocks; ++nb) {
+              wait(b_full + ring.idx, ring.ph);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t slot = slot0 + ring.idx * (kTrSlot >> 4);
+              const uint32_t d = tmem + nb * 128;
+              if constexpr (FP8) {
+                const uint32_t bl = slot + (8192u >> 4 << 16);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                  for (int t = 0; t < kPTerms; ++t)
+                    tc_mma_pair<true>(d, p_lo + t * (8192 >> 4) + ks * 2, sdesc_hi(1024), bl + ks * (4096 >> 4), sdesc_hi(1024),
+                                      idesc(1, 0, 256, 1), k > k0 || ks > 0 || t > 0);
+              } else {
+                const int nc = v_cols(nb, 0);
+                const uint32_t id = nc == 2 ? idesc(1, 1, 256, 1) : idesc(1, 1, 128, 1);
+                // columns of the slot LBO apart, 8-token groups SBO apart; a step is 16 tokens
+                const bool paired = nc == 2 && !tail;
+                const uint32_t bl = slot + (paired ? 1024u >> 4 << 16 : 8192u >> 4 << 16);
+                const uint32_t bh = paired ? sdesc_hi(2048) : sdesc_hi(1024), step = paired ? 4096u >> 4 : 2048u >> 4;
+                const uint32_t pl = p_lo + th * (8192 >> 4);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                  tc_mma_pair<false>(d, pl + ks * 2, sdesc_hi(1024), bl + ks * step, bh, id, k > k0 || th > 0 || ks > 0);
+              }
+              tc_commit_pair(bar(b_empty + ring.idx));
+              ring.next(m.nslots);
+            }
+          if (ok) tc_commit_pair(bar(b_odone));
+          ++jp;
+        }
+        ++seg;
+      }
+      volatile int never = 0;  // drain before TMEM is released
+      __syncwarp();
+      tc_commit_pair(bar(b_fin));
+      mbar_wait(bar(b_fin), 0, &never, nullptr, 100000000ull);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp >= kTrFacWarp) {
     // ---------------------------------------------------------------- score factors, a token per thread
-    const int ft = threadIdx.x - 128;
+    const int ft = threadIdx.x - 32 * kTrFacWarp;
     const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
     const float gs = a.sm_scale * kscale * (a.logit_cap > 0.f ? 1.f : kLog2e);
     const int rb = !FP8 || a.rms_mode == 2 ? 2 : 1;  // bytes per divisor
@@ -518,27 +523,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           fac[h * kTrFacPitch + ft] = f;
         }
         const unsigned v = __ballot_sync(0xffffffffu, here);
-        if (lane == 0) valid_s[warp - 4] = v;
+        if (lane == 0) valid_s[warp - kTrFacWarp] = v;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(b_facfull));
       }
     }
   } else {
     // ---------------------------------------------------------------- softmax and epilogue
-    const int l = threadIdx.x;              // TMEM lane
-    const int i = l & 63, half = l >> 6;    // row of the CTA; half of the tile's tokens, of a block's dims
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const int l = threadIdx.x & 127, wg = warp >> 2;  // TMEM lane; which 32 of its 64 columns
+    const int i = l & 63, half = l >> 6;              // row of the CTA; half of the tile's tokens, of a block's dims
+    const int quarter = 2 * half + wg;                // this thread's 32 tokens of the tile
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int x_row = g * 128 + (int)cta * 64 + i;
     const bool live = x_row < m.rows;
     const int node = live ? x_row / a.heads : 0, h = live ? x_row - node * a.heads : 0;
-    const float* fac_row = fac + h * kTrFacPitch + half * 64;
+    const float* fac_row = fac + h * kTrFacPitch + quarter * 32;
     const bool cap = a.logit_cap > 0.f;
     const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
     const uint32_t sempty0 = leader(b_sempty), pfull0 = leader(b_pfull), ofree0 = leader(b_ofree);
+    const uint32_t prow = pbuf + i * 128;
     SegCursor cur{req0, lo, hi};
     int r, k0, k1, plo, phi;
     uint32_t jt = 0;
-    // ok: this warp's waits so far; dead: the four warps have agreed (in a group barrier) to leave
+    // ok: this warp's waits so far; dead: the warps have agreed (in a group barrier) to leave
     bool ok = true, dead = false;
     while (!dead && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
       const int ctx = tree_ctx(a, r);
@@ -549,13 +556,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       float m_ref = -INFINITY, l_part = 0.f;
       for (int k = k0; k < k1; ++k, ++jt) {
         const uint32_t sb = jt & 1;
-        float x[64];
+        float x[32];
         ok = ok && mbar_wait(bar(b_sfull + sb), (jt >> 1) & 1, abort_flag, m.status);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           tc_fence_after();
-          tmem_ld32(tmem + lane_base + col_s + sb * 64, x);
-          tmem_ld32(tmem + lane_base + col_s + sb * 64 + 32, x + 32);
+          tmem_ld32(tmem + lane_base + col_s + sb * 64 + wg * 32, x);
           tmem_wait_ld();
           tc_fence_before();
           __syncwarp();
@@ -563,68 +569,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           ok = mbar_wait(bar(b_facfull), jt & 1, abort_flag, m.status);
           ok = __all_sync(0xffffffffu, ok);
         }
-        uint64_t vis = 0;
+        uint32_t vis = 0;
         if (ok) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
+          for (int e = 0; e < 32; e += 4) {
             const float4 f = *reinterpret_cast<const float4*>(fac_row + e);
             x[e] *= f.x;
             x[e + 1] *= f.y;
             x[e + 2] *= f.z;
             x[e + 3] *= f.w;
           }
-          vis = (uint64_t)valid_s[2 * half] | (uint64_t)valid_s[2 * half + 1] << 32;
+          vis = valid_s[quarter];
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(b_facfree));
         }
         if constexpr (FP8) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e) x[e] *= q_inv;
+          for (int e = 0; e < 32; ++e) x[e] *= q_inv;
         }
         if (cap) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e) x[e] = a.logit_cap * tanhf(x[e] / a.logit_cap) * kLog2e;
+          for (int e = 0; e < 32; ++e) x[e] = a.logit_cap * tanhf(x[e] / a.logit_cap) * kLog2e;
         }
         // tokens this row sees: committed ones, and drafts of its mask
-        const int64_t b0 = (int64_t)k * kTile + half * 64;
-        if (b0 + 64 > ctx || mask == 0) {
-          const int64_t nc = (int64_t)ctx - b0;  // committed tokens of this half
-          uint64_t see = nc <= 0 ? 0ull : nc >= 64 ? ~0ull : (1ull << nc) - 1;
+        const int nc = ctx - (k * kTile + quarter * 32);  // committed tokens from this thread's first on
+        if (nc < 32 || mask == 0) {
+          uint32_t see = nc <= 0 ? 0u : nc >= 32 ? ~0u : (1u << nc) - 1;
           if (nc >= 0)
-            see |= nc < 64 ? mask << nc : 0ull;
+            see |= nc < 32 ? (uint32_t)(mask << nc) : 0u;
           else
-            see |= -nc < 64 ? mask >> -nc : 0ull;
-          vis &= mask == 0 ? 0ull : see;
+            see |= -nc < 64 ? (uint32_t)(mask >> -nc) : 0u;
+          vis &= mask == 0 ? 0u : see;
         }
         float mx = -INFINITY;
-        if (vis == ~0ull) {
+        if (vis == ~0u) {
+          float mq[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-          for (int e = 0; e < 64; ++e) mx = fmaxf(mx, x[e]);
+          for (int e = 4; e < 32; ++e) mq[e & 3] = fmaxf(mq[e & 3], x[e]);
+          mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
         } else {
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
+          for (int e = 0; e < 32; ++e) {
             if (!(vis >> e & 1)) x[e] = -INFINITY;
             mx = fmaxf(mx, x[e]);
           }
         }
         bool need = mx > m_ref + kThr;
         // one group barrier per tile reduces the rescale test and any failed wait
-        need = named_bar_or(1, 128, need || !ok);
+        need = named_bar_or(1, kTrSoft, need || !ok);
         if (need) {
-          dead = named_bar_or(1, 128, !ok);
+          dead = named_bar_or(1, kTrSoft, !ok);
           if (dead) break;
-          red[l] = mx;
-          named_bar_sync(1, 128);
-          const float mn = fmaxf(m_ref, fmaxf(mx, red[l ^ 64]));
+          red[quarter * 64 + i] = mx;
+          named_bar_sync(1, kTrSoft);
+          const float mn = fmaxf(fmaxf(fmaxf(red[i], red[64 + i]), fmaxf(red[128 + i], red[192 + i])), m_ref);
           const float al = mn == m_ref ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - mn);
           m_ref = mn;
           l_part *= al;
-          if (named_bar_or(1, 128, al != 1.f && k > k0)) {  // (red[] is free again)
+          if (named_bar_or(1, kTrSoft, al != 1.f && k > k0)) {  // (red[] is free again)
             ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
               tc_fence_after();
-              for (int c = 0; c < m.o_cols; c += 16) {
+              for (int c = wg * 16; c < m.o_cols; c += 32) {  // the warpgroups take every other 16 columns
                 float o[16];
                 tmem_ld16(tmem + lane_base + c, o);
                 tmem_wait_ld();
@@ -638,51 +645,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           }
         }
         // P = 2^(x - m): nothing where the row sees nothing (m = -inf)
-        const float sub = m_ref == -INFINITY && vis != ~0ull ? 0.f : m_ref - kShift;
-        uint32_t w[FP8 ? 48 : 32];
+        const float sub = m_ref == -INFINITY && vis != ~0u ? 0.f : m_ref - kShift;
+        uint32_t w[FP8 ? 24 : 16];
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (!FP8) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) {
+          for (int e = 0; e < 32; e += 2) {
             const float pa = ex2_approx(x[e] - sub), pb = ex2_approx(x[e + 1] - sub);
-            l_part += pa + pb;
+            ls[e & 2] += pa;
+            ls[(e & 2) + 1] += pb;
             const __nv_bfloat162 b = __floats2bfloat162_rn(pa, pb);
             w[e >> 1] = *reinterpret_cast<const uint32_t*>(&b);
           }
         } else {
+          // e5m2 is the upper byte of f16: P goes to f16, is rounded there to 9 significant bits, and the
+          // three terms are what its upper byte holds, three bits at a time (exact subtractions).
+          // A NaN's bits may wrap in the rounding; it is in l already.
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            w[q] = w[16 + q] = w[32 + q] = 0u;
+          for (int q = 0; q < 8; ++q) {
+            uint32_t v[2];
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              float2 v = make_float2(ex2_approx(x[4 * q + e] - sub), ex2_approx(x[4 * q + e + 1] - sub));
-              l_part += v.x + v.y;
+            for (int e = 0; e < 2; ++e) {
+              const float pa = ex2_approx(x[4 * q + 2 * e] - sub), pb = ex2_approx(x[4 * q + 2 * e + 1] - sub);
+              ls[2 * e] += pa;
+              ls[2 * e + 1] += pb;
+              const __half2 hv = __floats2half2_rn(pa, pb);
+              v[e] = (*reinterpret_cast<const uint32_t*>(&hv) + 0x00020002u) & 0xfffcfffcu;
+            }
 #pragma unroll
-              for (int t = 0; t < kPTerms; ++t) {
-                const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E5M2);
-                w[16 * t + q] |= (uint32_t)b << (8 * e);
-                const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E5M2)));
-                v.x -= f.x;
-                v.y -= f.y;
+            for (int t = 0; t < kPTerms; ++t) {
+              w[8 * t + q] = __byte_perm(v[0], v[1], 0x7531);  // the upper bytes of four values
+              if (t + 1 < kPTerms) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t top = v[e] & 0xff00ff00u;
+                  const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&v[e]), *reinterpret_cast<const __half2*>(&top));
+                  v[e] = *reinterpret_cast<const uint32_t*>(&rest);
+                }
               }
             }
           }
         }
+        l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         // the P buffer is free, and O at rest, once the previous tile's PV is done
         if (ok && jt > 0) ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-          const uint32_t prow = pbuf + i * 128;
           if constexpr (!FP8) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-              st_shared_v4(prow + half * 8192 + ((u ^ (i & 7)) << 4), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+            for (int u = 0; u < 4; ++u)
+              st_shared_v4(prow + half * 8192 + (((wg * 4 + u) ^ (i & 7)) << 4), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
           } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const uint32_t at = prow + (((half * 4 + u) ^ (i & 7)) << 4);
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t at = prow + (((quarter * 2 + u) ^ (i & 7)) << 4);
 #pragma unroll
               for (int t = 0; t < kPTerms; ++t)
-                st_shared_v4(at + t * 8192, w[16 * t + 4 * u], w[16 * t + 4 * u + 1], w[16 * t + 4 * u + 2], w[16 * t + 4 * u + 3]);
+                st_shared_v4(at + t * 8192, w[8 * t + 4 * u], w[8 * t + 4 * u + 1], w[8 * t + 4 * u + 2], w[8 * t + 4 * u + 3]);
             }
           }
           fence_proxy_async_smem();
@@ -694,11 +713,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       if (dead) break;
       // ---- O / l -> the output, or this range's piece of it
       ok = ok && mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
-      red[l] = l_part;
-      dead = named_bar_or(1, 128, !ok);
+      red[quarter * 64 + i] = l_part;
+      dead = named_bar_or(1, kTrSoft, !ok);
       if (dead) break;
       tc_fence_after();
-      const float lt = l_part + red[l ^ 64];
+      const float lt = (red[i] + red[64 + i]) + (red[128 + i] + red[192 + i]);
       const float inv = lt == 0.f ? 0.f : kscale / lt;
       const bool full = plo >= lo && phi <= hi;
       const int64_t piece = ((int64_t)(plo <= lo ? 2 * range : 2 * range + 1) * m.groups + g) * 128 + cta * 64 + i;
@@ -707,7 +726,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       for (int nb = 0; nb < v_blocks; ++nb) {
         const int cols = FP8 ? 128 : 64 * v_cols(nb, 0);  // dims of this block in a lane
         const int d0 = nb * 256 + half * cols;
-        for (int c = 0; c < cols; c += 16) {
+        for (int c = wg * 16; c < cols; c += 32) {
           float o[16];
           tmem_ld16(tmem + lane_base + nb * 128 + c, o);
           tmem_wait_ld();
@@ -735,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           }
         }
       }
-      if (live && half == 0) {
+      if (live && quarter == 0) {
         const float l2 = lt == 0.f ? -INFINITY : m_ref + log2f(lt) - kShift;
         if (!full)
           m.part_lse[piece] = l2;
@@ -743,7 +762,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           store_from_float(a.lse + (orow * a.lse_sr + h) * dt_size(a.lse_dtype), a.lse_dtype, l2 * kLn2);
       }
       tc_fence_before();
-      named_bar_sync(1, 128);  // red[] is read
+      named_bar_sync(1, kTrSoft);  // red[] is read
       if (lane == 0) mbar_arrive_cluster(ofree0);
     }
   }
@@ -751,7 +770,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves while the other may still signal it or read its tiles
-  if (warp == 9) {
+  if (warp == kTrMmaWarp) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
   }
@@ -761,12 +780,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
 // (request, query row).  Requests inside one range are final already.
 __global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, const TreeMma m) {
   const int r = blockIdx.x, x = blockIdx.y;
+  __shared__ int bnd[kMaxCtas + 1];
   const int plo = __ldg(m.prefix + r), phi = __ldg(m.prefix + r + 1);
+  for (int c = threadIdx.x; c <= m.ranges; c += 128) bnd[c] = __ldg(m.bounds + c);
+  __syncthreads();
   auto range_of = [&](int t) {  // the non-empty range that holds tile t
     int lo = 0, hi = m.ranges;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(m.bounds + mid) <= t)
+      if (bnd[mid] <= t)
         lo = mid;
       else
         hi = mid;
@@ -785,11 +807,11 @@ __global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, cons
     int np = 0;
     for (int b = c0; b <= c1; b += 32) {
       const int c = b + (int)threadIdx.x;
-      const bool in = c <= c1 && __ldg(m.bounds + c) < __ldg(m.bounds + c + 1);  // empty ranges wrote nothing
+      const bool in = c <= c1 && bnd[c] < bnd[c + 1];  // empty ranges wrote nothing
       const unsigned bal = __ballot_sync(0xffffffffu, in);
       if (in) {
         const int k = np + __popc(bal & ((1u << threadIdx.x) - 1));
-        const int slot = plo <= __ldg(m.bounds + c) ? 2 * c : 2 * c + 1;
+        const int slot = plo <= bnd[c] ? 2 * c : 2 * c + 1;
         at[k] = ((int64_t)slot * m.groups + g) * 128 + i;
         wts[k] = __ldg(m.part_lse + at[k]);
       }

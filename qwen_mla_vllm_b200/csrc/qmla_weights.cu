@@ -152,6 +152,7 @@ struct WeightMmaArgs {
   uint32_t nk, off_q, off_meta, off_bars;
   int units, base_b, skip;  // rms tail: 16-byte units read per token, first byte, bytes to skip
   int first;                // this pass applies the decay
+  int q_vec;
   int* status;
 };
 struct WeightMaps {
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(256) weights_prep_kernel(const WeightArgs a, c
   const int h = col / m.jn, j = m.j0 + col % m.jn;
   const bool live = h < a.heads;
   const int64_t row = (int64_t)r * a.qrows + j;
-  const QSource s{a.q, a.q_pe, a.q_sr, a.q_sh, a.qpe_sr, a.qpe_sh, a.q_dtype, a.rank, a.qk_dim};
+  const QSource s{a.q, a.q_pe, a.q_sr, a.q_sh, a.qpe_sr, a.qpe_sh, a.q_dtype, a.rank, a.qk_dim, m.q_vec};
   const float inv = write_q_row<FP8>(s, live ? row : -1, h, img + (int64_t)r * m.img_bytes, col, m.np, m.chunks, m.terms);
   if (lane == 0) {
     float* mt = meta + (int64_t)r * 3 * m.np;
@@ -545,6 +546,7 @@ int launch_mma(const qmla_weights_params* p, const WeightArgs& a, const WeightPl
   m.prefix = reinterpret_cast<const int32_t*>(ws + pl.ws_prefix);
   m.meta = reinterpret_cast<const float*>(ws + pl.ws_meta);
   m.img = ws + pl.ws_img;
+  m.q_vec = q_vec(a.q, a.q_sr, a.q_sh, a.q_pe, a.qpe_sr, a.qpe_sh, a.rank, a.qk_dim);
   WeightMaps maps;
   const cuuint64_t tok = p->kv_stride_token * es, page = p->kv_stride_page * es;
   const cuuint32_t col = 128 / es;
