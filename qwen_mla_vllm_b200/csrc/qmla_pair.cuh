@@ -20,35 +20,11 @@ __device__ __forceinline__ uint32_t map_cta(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
   return a;
 }
-// Arrive on an mbarrier of any CTA of the cluster (an address from map_cta).
+// Arrive on an mbarrier of any CTA of the cluster (an address from map_cta).  The default scope: what
+// such an arrival hands over here (TMEM read out, P in this CTA's own shared memory behind a proxy
+// fence) never leaves the CTA, and a cluster-scope release costs a memory barrier of ~1000 cycles.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity, uint32_t hint_ns) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(hint_ns)
-      : "memory");
-  return ok != 0;
-}
-// mbar_wait for a barrier that the peer CTA arrives on: acquires what it wrote before arriving.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                                  uint64_t limit_ns = 2000000000ull) {
-  if (mbar_try_wait_cluster(bar, parity, 0u)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (true) {
-    if (mbar_try_wait_cluster(bar, parity, 20000u)) return true;
-    if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > limit_ns) {
-      *abort_flag = 1;
-      if (status) atomicOr(status, QMLA_DEV_ERR_TIMEOUT);
-      return false;
-    }
-  }
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Tiled loads into this CTA's shared memory whose bytes are counted on an mbarrier of either CTA

@@ -257,7 +257,7 @@ struct TreePlan {
 };
 
 // Clusters of the tensor-core kernel that can be resident at once (asked once per device).
-template <bool FP8>
+template <bool FP8, int TERMS>
 int resident_clusters(int device) {
   static std::mutex mu;
   static std::map<int, int> known;
@@ -265,13 +265,13 @@ int resident_clusters(int device) {
   auto it = known.find(device);
   if (it != known.end()) return it->second;
   int n = 0;
-  if (cudaFuncSetAttribute(tree_mma_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem) == cudaSuccess) {
+  if (cudaFuncSetAttribute(tree_mma_kernel<FP8, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem) == cudaSuccess) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(2);
     cfg.blockDim = dim3(kTrThreads);
     cfg.dynamicSmemBytes = kMaxDynSmem;
-    if (cudaOccupancyMaxActiveClusters(&n, tree_mma_kernel<FP8>, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, tree_mma_kernel<FP8, TERMS>, &cfg) != cudaSuccess) n = 0;
   }
   known[device] = n;
   return n;
@@ -303,7 +303,9 @@ void plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
     if (m.units > 7 || m.base_b + 16 * m.units > p->kv_row_width * es) return;
   }
   const int64_t rows = (int64_t)p->num_nodes * p->num_heads;
-  const int clusters = fp8 ? resident_clusters<true>(p->device) : resident_clusters<false>(p->device);
+  const int dev = p->device;
+  const int clusters = fp8 ? (m.terms == 2 ? resident_clusters<true, 2>(dev) : resident_clusters<true, 3>(dev))
+                           : (m.terms == 1 ? resident_clusters<false, 1>(dev) : resident_clusters<false, 2>(dev));
   if (rows > (int64_t)128 * clusters) return;
   m.rows = (int)rows;
   m.groups = (int)((rows + 127) / 128);
@@ -434,7 +436,12 @@ int launch_tree_mma(const qmla_tree_params* p, const TreeArgs& a, const TreePlan
   const int64_t warps = (int64_t)p->num_reqs * (m.groups * 128 + kTrTail);
   if (warps / 8 + 1 > INT32_MAX) return QMLA_E_UNSUPPORTED;
   tree_prep_kernel<FP8><<<(unsigned)((warps + 7) / 8 + 1), 256, 0, st>>>(a, m);
-  tree_mma_kernel<FP8><<<2 * m.ranges * m.groups, kTrThreads, pl.smem, st>>>(maps, a, m);
+  const int grid = 2 * m.ranges * m.groups;
+  constexpr int T0 = FP8 ? 2 : 1;
+  if (m.terms == T0)
+    tree_mma_kernel<FP8, T0><<<grid, kTrThreads, pl.smem, st>>>(maps, a, m);
+  else
+    tree_mma_kernel<FP8, T0 + 1><<<grid, kTrThreads, pl.smem, st>>>(maps, a, m);
   tree_pieces_kernel<<<dim3(p->num_reqs, m.rows), 128, 0, st>>>(a, m);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
 }

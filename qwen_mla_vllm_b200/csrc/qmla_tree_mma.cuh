@@ -27,9 +27,9 @@
 // zeroed (prep kernel): a node that does not see such a token has P = 0 there, and 0 * NaN must not
 // reach it; a node that sees it has S = NaN already.
 //
-// Warps of a CTA: 0-7 softmax and epilogue (a thread owns 32 tokens of one row), 8-11 score factors
-// (1 / rms per token and head, a token per thread), 12 TMA loads, 13 MMA issue (leader) or the
-// announcement that Q has landed (peer).
+// Warps of a CTA: 0-7 softmax and epilogue (a thread owns 32 tokens of one row), 8-10 score factors
+// (1 / rms per token and head), 11 MMA issue (leader) or the announcement that Q has landed (peer), 12-15 TMA loads in turn: a warp spends 400 cycles or more on a slot's boxes
+// (16-token pages: four of 4 KB, ~50 cycles each past the first), four warps keep up with the ring.
 #pragma once
 #include "qmla_decode.cuh"
 #include "qmla_pair.cuh"
@@ -70,8 +70,8 @@ __device__ __forceinline__ int tree_ctx(const TreeArgs& a, int r) {
   return (int)min((int64_t)max(__ldg(a.ctx + r), 0), room);
 }
 
-constexpr int kTrSoftWarps = 8, kTrFacWarp = 8, kTrLoadWarp = 12, kTrMmaWarp = 13;
-constexpr int kTrThreads = 448;
+constexpr int kTrSoftWarps = 8, kTrFacWarp = 8, kTrFacWarps = 3, kTrMmaWarp = 11, kTrLoadWarp = 12, kTrLoadWarps = 4;
+constexpr int kTrThreads = 512;
 constexpr int kTrSoft = 32 * kTrSoftWarps;  // softmax threads
 constexpr int kTrRows = 64;          // query rows per CTA
 constexpr int kTrTail = 256;         // tokens of a request's copied tail (127 + 64 at most)
@@ -79,6 +79,12 @@ constexpr int kTrFacPitch = 132;     // floats between heads in the factor table
 constexpr int kTrMaxSlots = 10;
 constexpr uint32_t kTrSlot = 16384;
 constexpr int tr_p_bytes(bool fp8) { return fp8 ? 24576 : 16384; }  // P of a CTA's 64 rows x 128 tokens
+
+// Instruction descriptor of a paired M = 128 tile: 32-bit sums, A K-major, formats 0 = e4m3 (f16),
+// 1 = e5m2 (bf16); b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t tr_idesc(uint32_t fa, uint32_t fb, uint32_t N, uint32_t b_mn) {
+  return (1u << 4) | (fa << 7) | (fb << 10) | (b_mn << 16) | ((N >> 3) << 17) | ((128u >> 4) << 24);
+}
 
 struct TreeMma {
   int32_t* prefix;   // [reqs + 1] tiles
@@ -186,7 +192,8 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const TreeArgs a, const 
   for (int c = threadIdx.x; c <= m.ranges; c += 256) m.bounds[c] = range_bound(m.prefix, a.reqs, m.ranges, m.seg_cost, c);
 }
 
-template <bool FP8>
+// TERMS: terms of a query element (qmla_qimage.cuh).
+template <bool FP8, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     tree_mma_kernel(const __grid_constant__ TreeMaps maps, const TreeArgs a, const TreeMma m) {
   constexpr float kThr = FP8 ? 2.f : 8.f;    // log2 units a weight may exceed 1 by before O is rescaled
@@ -236,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     mbar_init(bar(b_qfull), 1);
     mbar_init(bar(b_qempty), 1);
     mbar_init(bar(b_qpeer), 1);
-    mbar_init(bar(b_facfull), 4);
+    mbar_init(bar(b_facfull), kTrFacWarps);
     mbar_init(bar(b_facfree), kTrSoftWarps);
     mbar_init(bar(b_fin), 1);
     *abort_flag = 0;
@@ -262,10 +269,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
   };
   auto v_col0 = [&](int nb, int c) -> int { return FP8 ? 2 * nb + c : 4 * nb + c * v_cols(nb, c); };
 
-  if (warp == kTrLoadWarp) {
+  if (warp >= kTrLoadWarp) {
     // ---------------------------------------------------------------- loads
-    // All lanes wait for a slot; lane 0 arms the leader's barrier for both CTAs' bytes; each of the
-    // first lanes issues one box.  What a box needs beside its column is worked out once per tile.
+    // The load warps take the slots in turn (no more warps than slots: a warp then filled the slot
+    // `warps` before this one, so the phase it waits for is never two behind).  All lanes wait; lane 0
+    // arms the leader's barrier for both CTAs' bytes; each of the first lanes issues one box.  What a
+    // box needs beside its column is worked out once per tile.
+    const uint32_t lw = warp - kTrLoadWarp, nlw = min((uint32_t)kTrLoadWarps, m.nslots);
+    uint32_t turn = lw < nlw ? 0u : 1000u;  // whose slot is next (a warp without slots never matches)
     const uint64_t pol = policy_evict_normal();
     const int run = m.run, khalf = 64 / run;  // boxes of a CTA's 64 tokens of K
     const int k_slots = (m.chunks + 1) / 2;
@@ -275,21 +286,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     const uint32_t k_wide = kb * run * 256, k_plain = kc * 8192 + kb * run * 128;
     SegCursor cur{req0, lo, hi};
     int r, k0, k1, plo, phi;
-    uint32_t seg = 0, armed = 0;
+    uint32_t seg = 0, count = 0;  // slots so far
     Ring ring;
     bool ok = true;
+    auto slot_mine = [&]() { return turn == lw; };
+    auto slot_next = [&]() {
+      ring.next(m.nslots);
+      ++count;
+      if (lw < nlw) turn = turn + 1 == nlw ? 0u : turn + 1;
+    };
     auto slot_begin = [&](uint32_t bytes) {
       ok = mbar_wait(bar(b_empty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && cta == 0 && lane == 0) mbar_expect_tx(bar(b_full + ring.idx), bytes);
     };
     while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-      if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_expect_tx(bar(b_qfull), m.img_bytes);
-        load_image(qbuf, m.img + (((int64_t)r * m.groups + g) * 2 + cta) * m.img_bytes, m.img_bytes, bar(b_qfull), pol);
+      if (lw == 0) {
+        if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(bar(b_qfull), m.img_bytes);
+          load_image(qbuf, m.img + (((int64_t)r * m.groups + g) * 2 + cta) * m.img_bytes, m.img_bytes, bar(b_qfull), pol);
+        }
       }
       ++seg;
       const int n = (int)tree_tokens(a, r);
@@ -313,7 +332,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
         if (k < k1) {  // K of tile k: this CTA's 64 tokens, two columns per slot
           const int kpg = __shfl_sync(0xffffffffu, pg, (int)cta * khalf + kb);
           const int ky = __shfl_sync(0xffffffffu, y, (int)cta * khalf + kb);
-          for (int s = 0; s < k_slots; ++s) {
+          for (int s = 0; s < k_slots; ++s, slot_next()) {
+            if (!slot_mine()) continue;
             const int c0 = 2 * s, nch = min(2, m.chunks - c0);
             slot_begin((uint32_t)nch * 2u * 8192u);
             if (!ok) break;
@@ -323,8 +343,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
             } else if (lane < khalf) {
               tma_load_5d_pair(slot + k_wide, &maps.wide, 0, 0, c0, ky >> 3, kpg, fb, pol);
             }
-            ++armed;
-            ring.next(m.nslots);
           }
         }
         if (k > k0 && ok) {  // V of tile k - 1: all its tokens, this CTA's half of the dims
@@ -334,7 +352,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           for (int th = 0; th < NV && ok; ++th) {
             const int vpg = __shfl_sync(0xffffffffu, pg_prev, th * khalf + vb);
             const int vy = __shfl_sync(0xffffffffu, y_prev, th * khalf + vb);
-            for (int nb = 0; nb < v_blocks; ++nb) {
+            for (int nb = 0; nb < v_blocks; ++nb, slot_next()) {
+              if (!slot_mine()) continue;
               const int nc = v_cols(nb, (int)cta), vc0 = v_col0(nb, (int)cta);
               constexpr int toks = kTile / NV;
               slot_begin((uint32_t)((v_cols(nb, 0) + v_cols(nb, 1)) * toks * 128));
@@ -351,8 +370,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
                 else
                   tma_load_3d_pair(slot + lane * run * 128, &maps.chunk, vc0 * E, vy, vpg, fb, pol);
               }
-              ++armed;
-              ring.next(m.nslots);
             }
           }
         }
@@ -362,10 +379,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     }
     if (!ok && lane == 0) {  // after an abort: wait (bounded) for the copies already issued
       volatile int never = 0;
-      if (cta == 0)
-        for (uint32_t p = armed > m.nslots ? armed - m.nslots : 0u; p < armed; ++p)
-          mbar_wait(bar(b_full + p % m.nslots), (p / m.nslots) & 1, &never, nullptr, 20000000ull);
-      if (seg > 0) mbar_wait(bar(b_qfull), (seg - 1) & 1, &never, nullptr, 20000000ull);
+      if (cta == 0 && lw < nlw)
+        for (uint32_t p = count > m.nslots ? count - m.nslots : 0u; p < count; ++p)
+          if (p % nlw == lw) mbar_wait(bar(b_full + p % m.nslots), (p / m.nslots) & 1, &never, nullptr, 20000000ull);
+      if (lw == 0 && seg > 0) mbar_wait(bar(b_qfull), (seg - 1) & 1, &never, nullptr, 20000000ull);
     }
     __syncwarp();
   } else if (warp == kTrMmaWarp) {
@@ -381,9 +398,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
         ++seg;
       }
     } else {
-      auto idesc = [](uint32_t fa, uint32_t fb, uint32_t N, uint32_t b_mn) {
-        return (1u << 4) | (fa << 7) | (fb << 10) | (b_mn << 16) | ((N >> 3) << 17) | ((128u >> 4) << 24);
-      };
       const uint32_t q_lo = sdesc_lo(qbuf, 16), p_lo = sdesc_lo(pbuf, 16);
       const uint32_t qt16 = (uint32_t)(m.chunks * kTrRows * 128) >> 4;
       const uint32_t slot0 = sbase >> 4;
@@ -391,36 +405,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       uint32_t js = 0, jp = 0;  // tiles scored / accumulated so far
       Ring ring;
       auto wait = [&](uint32_t b, uint32_t ph) {  // the whole warp
-        ok = ok && mbar_wait_cluster(bar(b), ph, abort_flag, m.status);
+        ok = ok && mbar_wait(bar(b), ph, abort_flag, m.status);
         ok = __all_sync(0xffffffffu, ok);
+      };
+      // The slot at the head of the ring.  Its barrier is tried before the MMAs of the slot before it
+      // are issued, so that the answer is there when they are.
+      bool peek = false;
+      auto slot_wait = [&]() {
+        if (!__all_sync(0xffffffffu, peek)) wait(b_full + ring.idx, ring.ph);
+        tc_fence_after();
+      };
+      auto slot_peek_next = [&]() {
+        Ring nx = ring;
+        nx.next(m.nslots);
+        peek = mbar_try_wait(bar(b_full + nx.idx), nx.ph);
+      };
+      auto slot_done = [&]() {
+        tc_commit_pair(bar(b_empty + ring.idx));
+        ring.next(m.nslots);
       };
       auto qk = [&]() {
         const uint32_t sb = js & 1;
         if (js >= 2) wait(b_sempty + sb, ((js - 2) >> 1) & 1);
         const uint32_t d = tmem + col_s + sb * 64;
-        for (int s = 0; s < k_slots; ++s) {
-          wait(b_full + ring.idx, ring.ph);
+        uint32_t a_lo = q_lo;
+        for (int s = 0; s < k_slots; ++s, a_lo += 2 * kTrRows * 128 >> 4) {
+          slot_wait();
           if (!ok) return;
-          tc_fence_after();
+          slot_peek_next();
+          // column ci of the slot: 8 KB on (plain), or between the 8-row groups
           const bool plain = 2 * s + 2 > m.full_chunks;
-          const bool two = 2 * s + 1 < m.chunks;
-          // column ci of the slot: 8 KB on, or between the 8-row groups
           const uint32_t b_lo = slot0 + ring.idx * (kTrSlot >> 4) + (1u << 16), b_hi = plain ? sdesc_hi(1024) : sdesc_hi(2048);
           const uint32_t b_col = plain ? 8192 >> 4 : 1024 >> 4;
-          const uint32_t a_lo = q_lo + (uint32_t)s * (2 * kTrRows * 128 >> 4);
+          const bool two = 2 * s + 1 < m.chunks;
 #pragma unroll
           for (int ci = 0; ci < 2; ++ci) {
-            if (ci == 1 && !two) break;
-            for (int t = 0; t < m.terms; ++t) {
-              const uint32_t id = FP8 ? idesc(q_term_format(t), 0, 128, 0) : idesc(1, 1, 128, 0);
-              const uint32_t al = a_lo + ci * (kTrRows * 128 >> 4) + t * qt16, bl = b_lo + ci * b_col;
+            if (ci == 0 || two) {
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                tc_mma_pair<FP8>(d, al + ks * 2, sdesc_hi(1024), bl + ks * 2, b_hi, id, (s | ci | t | ks) != 0);
+              for (int t = 0; t < TERMS; ++t) {
+                constexpr uint32_t id0 = tr_idesc(0, 0, 128, 0), id1 = tr_idesc(1, 0, 128, 0), idb = tr_idesc(1, 1, 128, 0);
+                const uint32_t al = a_lo + ci * (kTrRows * 128 >> 4) + t * qt16, bl = b_lo + ci * b_col;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                  tc_mma_pair<FP8>(d, al + ks * 2, sdesc_hi(1024), bl + ks * 2, b_hi, !FP8 ? idb : t == 0 ? id0 : id1,
+                                   ci + t + ks > 0 ? 1u : (uint32_t)s);
+              }
             }
           }
-          tc_commit_pair(bar(b_empty + ring.idx));
-          ring.next(m.nslots);
+          slot_done();
         }
         tc_commit_pair(bar(b_sfull + sb));
         ++js;
@@ -439,11 +471,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           wait(b_pfull, jp & 1);
           if (k == k0 && seg > 0) wait(b_ofree, (seg - 1) & 1);
           const bool tail = k >= tail_tile;
+          const uint32_t acc0 = k > k0;
           for (int th = 0; th < NV && ok; ++th)
             for (int nb = 0; nb < v_blocks; ++nb) {
-              wait(b_full + ring.idx, ring.ph);
+              slot_wait();
               if (!ok) break;
-              tc_fence_after();
+              // (the slot after a segment's last V belongs to the next segment's K: not tried here)
+              if (th + 1 < NV || nb + 1 < v_blocks || k + 1 < k1)
+                slot_peek_next();
+              else
+                peek = false;
               const uint32_t slot = slot0 + ring.idx * (kTrSlot >> 4);
               const uint32_t d = tmem + nb * 128;
               if constexpr (FP8) {
@@ -453,21 +490,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
 #pragma unroll
                   for (int t = 0; t < kPTerms; ++t)
                     tc_mma_pair<true>(d, p_lo + t * (8192 >> 4) + ks * 2, sdesc_hi(1024), bl + ks * (4096 >> 4), sdesc_hi(1024),
-                                      idesc(1, 0, 256, 1), k > k0 || ks > 0 || t > 0);
+                                      tr_idesc(1, 0, 256, 1), ks + t > 0 ? 1u : acc0);
               } else {
                 const int nc = v_cols(nb, 0);
-                const uint32_t id = nc == 2 ? idesc(1, 1, 256, 1) : idesc(1, 1, 128, 1);
+                const uint32_t id = nc == 2 ? tr_idesc(1, 1, 256, 1) : tr_idesc(1, 1, 128, 1);
                 // columns of the slot LBO apart, 8-token groups SBO apart; a step is 16 tokens
                 const bool paired = nc == 2 && !tail;
                 const uint32_t bl = slot + (paired ? 1024u >> 4 << 16 : 8192u >> 4 << 16);
                 const uint32_t bh = paired ? sdesc_hi(2048) : sdesc_hi(1024), step = paired ? 4096u >> 4 : 2048u >> 4;
-                const uint32_t pl = p_lo + th * (8192 >> 4);
+                const uint32_t pl = p_lo + th * (8192 >> 4), acc1 = acc0 | (uint32_t)th;
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
-                  tc_mma_pair<false>(d, pl + ks * 2, sdesc_hi(1024), bl + ks * step, bh, id, k > k0 || th > 0 || ks > 0);
+                  tc_mma_pair<false>(d, pl + ks * 2, sdesc_hi(1024), bl + ks * step, bh, id, ks > 0 ? 1u : acc1);
               }
-              tc_commit_pair(bar(b_empty + ring.idx));
-              ring.next(m.nslots);
+              slot_done();
             }
           if (ok) tc_commit_pair(bar(b_odone));
           ++jp;
@@ -481,49 +517,92 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     }
     __syncwarp();
   } else if (warp >= kTrFacWarp) {
-    // ---------------------------------------------------------------- score factors, a token per thread
-    const int ft = threadIdx.x - 32 * kTrFacWarp;
+    // ---------------------------------------------------------------- score factors
+    // A work item is a 16-byte unit of one token's divisors: 8 heads (two bytes each) or 16 (one byte),
+    // unpacked in registers.  A tile's units are loaded before the table is free.
+    constexpr int kThreads = 32 * kTrFacWarps, kBatch = 4;
+    const int ft = threadIdx.x - 32 * kTrFacWarp, fw = warp - kTrFacWarp;
     const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
     const float gs = a.sm_scale * kscale * (a.logit_cap > 0.f ? 1.f : kLog2e);
-    const int rb = !FP8 || a.rms_mode == 2 ? 2 : 1;  // bytes per divisor
+    const bool two = !FP8 || a.rms_mode == 2;      // bytes per divisor
+    const bool split = two && (m.skip & 1);        // raw bytes at an odd offset: a divisor may span two units
+    const int items = kTile * (split ? a.heads : m.units);
+    auto factor = [&](uint32_t bits) -> float {
+      if (FP8 && a.rms_mode == 3) return gs * ex2_approx(3.0f - (float)bits * (6.0f / 255.0f));
+      const float rv = two ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits)) : e4m3_to_f32((uint8_t)bits) * kscale;
+      return rv > 0.f ? __fdividef(gs, rv) : gs;
+    };
     SegCursor cur{req0, lo, hi};
     int r, k0, k1, plo, phi;
     uint32_t jt = 0;
     bool ok = true;
     while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-      const int64_t n = tree_tokens(a, r);
+      const int n = (int)tree_tokens(a, r);
+      const int32_t* bt = a.bt + r * a.bt_stride;
+      // row of token t of tile k, or null when there is none
+      auto row_of = [&](int k, int t) -> const uint8_t* {
+        const uint32_t tok = (uint32_t)k * kTile + t;
+        if (tok >= (uint32_t)n) return nullptr;
+        const uint32_t pi = tok / (uint32_t)a.page_size;
+        const int pg = __ldg(bt + pi);
+        if (pg < 0 || pg >= a.num_pages) return nullptr;
+        return a.cache + (int64_t)pg * a.page_b + (tok - pi * (uint32_t)a.page_size) * a.tok_b;
+      };
       for (int k = k0; k < k1 && ok; ++k, ++jt) {
-        const int64_t t = (int64_t)k * kTile + ft;
-        alignas(16) uint8_t tailb[16 * 7];
-        bool here = false;
-        if (t < n) {
-          const int pg = __ldg(a.bt + r * a.bt_stride + t / a.page_size);
-          here = pg >= 0 && pg < a.num_pages;
-          if (here) {
-            const uint8_t* p = a.cache + (int64_t)pg * a.page_b + t % a.page_size * a.tok_b + m.base_b;
-            for (int u = 0; u < m.units; ++u) reinterpret_cast<uint4*>(tailb)[u] = __ldg(reinterpret_cast<const uint4*>(p) + u);
-          }
+        unsigned valid[2];  // tokens 32 fw .. and 32 (fw + 3) ..
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int t = (fw + q * kTrFacWarps) * 32 + lane;
+          valid[q] = __ballot_sync(0xffffffffu, t < kTile && row_of(k, t) != nullptr);
         }
+        uint4 v[kBatch];
+        auto load = [&](int i0) {
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int i = i0 + b * kThreads + ft;
+            v[b] = make_uint4(0u, 0u, 0u, 0u);
+            if (i >= items || split) continue;
+            const uint8_t* p = row_of(k, i & (kTile - 1));
+            if (p) v[b] = __ldg(reinterpret_cast<const uint4*>(p + m.base_b) + (i >> 7));
+          }
+        };
+        load(0);
         if (jt > 0) ok = mbar_wait(bar(b_facfree), (jt - 1) & 1, abort_flag, m.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        for (int h = 0; h < a.heads; ++h) {
-          float f = gs;
-          if (m.units > 0 && here) {
-            const uint8_t* b = tailb + m.skip + rb * h;
-            const uint32_t bits = rb == 1 ? *b : (uint32_t)b[0] | (uint32_t)b[1] << 8;
-            if (FP8 && a.rms_mode == 3) {
-              f *= ex2_approx(3.0f - (float)bits * (6.0f / 255.0f));
+        if (lane == 0) {
+          valid_s[fw] = valid[0];
+          if (fw + kTrFacWarps < 4) valid_s[fw + kTrFacWarps] = valid[1];
+        }
+        for (int i0 = 0; i0 < items; i0 += kBatch * kThreads) {
+          if (i0 > 0) load(i0);
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int i = i0 + b * kThreads + ft;
+            if (i >= items) continue;
+            const int t = i & (kTile - 1), u = i >> 7;
+            const uint32_t w[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+            if (split) {
+              const uint8_t* p = row_of(k, t);
+              if (p) p += m.base_b + m.skip + 2 * u;
+              fac[u * kTrFacPitch + t] = p ? factor((uint32_t)__ldg(p) | (uint32_t)__ldg(p + 1) << 8) : gs;
+            } else if (two) {
+              const int h0 = (16 * u - m.skip) / 2;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (h0 + e >= 0 && h0 + e < a.heads)
+                  fac[(h0 + e) * kTrFacPitch + t] = factor((w[e >> 1] >> (16 * (e & 1))) & 0xffffu);
             } else {
-              const float rv = (!FP8 || a.rms_mode == 2) ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits))
-                                                         : e4m3_to_f32((uint8_t)bits) * kscale;
-              f = rv > 0.f ? __fdividef(f, rv) : f;
+              const int h0 = 16 * u - m.skip;
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (h0 + e >= 0 && h0 + e < a.heads)
+                  fac[(h0 + e) * kTrFacPitch + t] = factor((w[e >> 2] >> (8 * (e & 3))) & 0xffu);
             }
           }
-          fac[h * kTrFacPitch + ft] = f;
         }
-        const unsigned v = __ballot_sync(0xffffffffu, here);
-        if (lane == 0) valid_s[warp - kTrFacWarp] = v;
+        if (items == 0)  // no divisors
+          for (int i = ft; i < kTile * a.heads; i += kThreads) fac[(i >> 7) * kTrFacPitch + (i & (kTile - 1))] = gs;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(b_facfull));
       }
