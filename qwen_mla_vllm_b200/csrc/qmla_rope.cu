@@ -23,9 +23,10 @@ using namespace qmla;
 
 namespace {
 
-constexpr int kRotThreads = 128;
-constexpr int kMaxRot = 512;           // dims of one rotated block
-constexpr int kStageBytes = 16 * 1024;  // staged elements of a block at most
+constexpr int kRotThreads = 256;
+constexpr int kRotWarps = kRotThreads / 32;
+constexpr int kMaxRot = 512;            // dims of one rotated block
+constexpr int kStageBytes = 16 * 1024;  // one staged segment at most
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -66,38 +67,33 @@ __device__ __forceinline__ int64_t position(const RotAngles& g, int64_t tok) {
                    : (int64_t)__ldg(reinterpret_cast<const int*>(g.pos) + tok);
 }
 
-// tab[w] = (cos, signed sin) of window dim w, so that out[w] = x[w] * tab.x + x[partner] * tab.y.
-__device__ __forceinline__ void fill_table(float2* tab, const RotAngles& g, int rot, int64_t pos, int i) {
+// (cos, sin) of pair i at a position, scaled; the adjoint turns the other way.
+__device__ __forceinline__ float2 turn_of(const RotAngles& g, int64_t pos, int i) {
   const uint64_t phase = (uint64_t)pos * (uint64_t)__ldg(reinterpret_cast<const long long*>(g.steps) + i);
   const float t = (float)(int32_t)(phase >> 32) * 4.656612873077393e-10f;  // 2^-31: half turns
   float s, c;
   sincospif(t, &s, &c);
-  s *= g.adjoint ? -g.scale : g.scale;
-  c *= g.scale;
-  const int a = g.interleaved ? 2 * i : i, b = g.interleaved ? 2 * i + 1 : i + rot / 2;
-  tab[a] = make_float2(c, -s);
-  tab[b] = make_float2(c, s);
+  return make_float2(c * g.scale, s * (g.adjoint ? -g.scale : g.scale));
 }
 
-__device__ __forceinline__ int partner(int w, int rot, int interleaved) {
-  const int h = rot >> 1;
-  return interleaved ? w ^ 1 : (w < h ? w + h : w - h);
+// Window pair j -> (offset of its first element in a head, pair of its block).
+__device__ __forceinline__ uint32_t pair_entry(const RotSpan& s, int interleaved, int j) {
+  const int half = s.rot >> 1, blk = j / half, i = j - blk * half;
+  return (uint32_t)(s.start + blk * s.rot + (interleaved ? 2 * i : i)) | (uint32_t)i << 16;
 }
 
-// Rotates segments [seg0, seg0 + nseg) of tokens [tok0, tok0 + ntok).  The segments are staged in
-// shared memory before any is written: the partner of an element may sit anywhere in the window
-// (58 dims turn as halves of 29), so out may be x itself, and global accesses are whole 16-byte
-// units (VEC) whatever the window's alignment.  Units belong to a thread in the order they are
-// loaded, all loads of a thread in flight at once.
+// Rotates segments [seg0, seg0 + nseg) of tokens [tok0, tok0 + ntok) by way of shared memory: loaded
+// and stored in whole 16-byte units (VEC) whatever the window's alignment (58 dims turn as halves of 29),
+// turned in place in between, a warp per head and a lane per pair.  Every element is staged before any
+// is written, so out may be x itself.  `table`: pair_entry of the window's pairs; `turns`: [ntok][rot / 2];
+// both are written before the call, the barrier below makes them visible.
 template <typename T, bool VEC>
-__device__ __forceinline__ void rotate_segments(const RotSpan& s, int interleaved, const float2* tab,
-                                                uint8_t* stage, int64_t tok0, int ntok, int seg0,
+__device__ __forceinline__ void rotate_segments(const RotSpan& s, int interleaved, const uint32_t* table,
+                                                const float2* turns, uint8_t* stage, int64_t tok0, int ntok, int seg0,
                                                 int nseg) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   const int ups = s.len / V;  // units per segment
   const int total = ntok * nseg * ups;
-  const int win = s.blocks * s.rot;
-  const T* st = reinterpret_cast<const T*>(stage);
 #pragma unroll 4
   for (int u = threadIdx.x; u < total; u += kRotThreads) {
     const int r = u / ups, k = u - r * ups;
@@ -109,41 +105,32 @@ __device__ __forceinline__ void rotate_segments(const RotSpan& s, int interleave
       reinterpret_cast<T*>(stage)[u] = *reinterpret_cast<const T*>(p);
   }
   __syncthreads();
-#pragma unroll 2
+  const int half = s.rot >> 1, pairs = s.blocks * half;
+  const int per_tok = nseg * (s.len / s.period), rows = ntok * per_tok;  // heads
+  const int dist = interleaved ? 1 : half;
+  for (int row = threadIdx.x >> 5; row < rows; row += kRotWarps) {
+    T* head = reinterpret_cast<T*>(stage) + row * s.period;
+    const float2* tb = turns + (row / per_tok) * half;
+#pragma unroll 4
+    for (int j = threadIdx.x & 31; j < pairs; j += 32) {
+      const uint32_t e = table[j];
+      const float2 cs = tb[e >> 16];
+      T* pa = head + (e & 0xffffu);
+      const float x = to_f32(pa[0]), y = to_f32(pa[dist]);
+      pa[0] = from_f32<T>(x * cs.x - y * cs.y);
+      pa[dist] = from_f32<T>(y * cs.x + x * cs.y);
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
   for (int u = threadIdx.x; u < total; u += kRotThreads) {
     const int r = u / ups, k = u - r * ups;
     const int t = r / nseg, sg = r - t * nseg;
-    const T* row = st + (int64_t)r * s.len;
-    int e = k * V;
-    int head = e / s.period;
-    int d = e - head * s.period;
-    int w = d - s.start;  // dim of the window, then of its block
-    if (w >= 0 && w < win) w %= s.rot;
-    const float2* tb = tab + t * s.rot;
-    alignas(16) T v[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const T own = row[e];
-      if (d >= s.start && d < s.start + win) {
-        const float2 cs = tb[w];
-        const float other = to_f32(row[e - w + partner(w, s.rot, interleaved)]);
-        v[i] = from_f32<T>(to_f32(own) * cs.x + other * cs.y);
-      } else {
-        v[i] = own;
-      }
-      ++e;
-      if (++d == s.period) {
-        d = 0;
-        w = -s.start;
-      } else if (++w == s.rot) {
-        w = 0;
-      }
-    }
     uint8_t* p = s.out + (tok0 + t) * s.o_st + (int64_t)(seg0 + sg) * s.o_ss + (int64_t)k * V * sizeof(T);
     if constexpr (VEC)
-      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+      *reinterpret_cast<uint4*>(p) = reinterpret_cast<const uint4*>(stage)[u];
     else
-      *reinterpret_cast<T*>(p) = v[0];
+      *reinterpret_cast<T*>(p) = reinterpret_cast<const T*>(stage)[u];
   }
 }
 
@@ -151,17 +138,72 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotSpan s, const RotAngles g,
                                                              int64_t n, int tpb, int spb) {
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* tab = reinterpret_cast<float2*>(smem);
-  uint8_t* stage = smem + ((tpb * s.rot * 8 + 15) & ~15);
+  const int half = s.rot >> 1, pairs = s.blocks * half;
+  float2* turns = reinterpret_cast<float2*>(smem);
+  uint32_t* table = reinterpret_cast<uint32_t*>(smem + tpb * half * 8);
+  uint8_t* stage = smem + ((tpb * half * 8 + pairs * 4 + 15) & ~15);
   const int64_t tok0 = (int64_t)blockIdx.x * tpb;
   const int ntok = (int)min((int64_t)tpb, n - tok0);
   const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
-  const int half = s.rot >> 1;
   for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
     const int t = i / half, k = i - t * half;
-    fill_table(tab + t * s.rot, g, s.rot, position(g, tok0 + t), k);
+    turns[i] = turn_of(g, position(g, tok0 + t), k);
   }
-  rotate_segments<T, VEC>(s, g.interleaved, tab, stage, tok0, ntok, seg0, nseg);
+  for (int j = threadIdx.x; j < pairs; j += kRotThreads) table[j] = pair_entry(s, g.interleaved, j);
+  rotate_segments<T, VEC>(s, g.interleaved, table, turns, stage, tok0, ntok, seg0, nseg);
+}
+
+// Pairs side by side within 16-byte units: nothing is staged, a thread turns the units it loads, four
+// in flight.
+template <typename T>
+__global__ void __launch_bounds__(kRotThreads) rotary_pairs_kernel(const RotSpan s, const RotAngles g,
+                                                                   int64_t n, int tpb, int spb) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int V = 16 / (int)sizeof(T), U = 4;
+  float2* turns = reinterpret_cast<float2*>(smem);
+  const int half = s.rot >> 1, win = s.blocks * s.rot;
+  const int64_t tok0 = (int64_t)blockIdx.x * tpb;
+  const int ntok = (int)min((int64_t)tpb, n - tok0);
+  const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
+  const int ups = s.len / V, total = ntok * nseg * ups;
+  for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
+    const int t = i / half, k = i - t * half;
+    turns[i] = turn_of(g, position(g, tok0 + t), k);
+  }
+  __syncthreads();
+  for (int u0 = threadIdx.x; u0 < total; u0 += U * kRotThreads) {
+    uint4 raw[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int u = u0 + q * kRotThreads;
+      if (u < total) {
+        const int r = u / ups, k = u - r * ups, t = r / nseg;
+        raw[q] = *reinterpret_cast<const uint4*>(s.x + (tok0 + t) * s.x_st + (int64_t)(seg0 + r - t * nseg) * s.x_ss + (int64_t)k * 16);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int u = u0 + q * kRotThreads;
+      if (u < total) {
+        const int r = u / ups, k = u - r * ups, t = r / nseg;
+        T* v = reinterpret_cast<T*>(&raw[q]);
+        const float2* tb = turns + t * half;
+        const int d0 = k * V - s.start;  // window dim of the unit's first element (even)
+        int w = d0 >= 0 ? d0 % s.rot : 0;
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          if (d0 + i >= 0 && d0 + i < win) {
+            const float2 cs = tb[w >> 1];
+            const float x = to_f32(v[i]), y = to_f32(v[i + 1]);
+            v[i] = from_f32<T>(x * cs.x - y * cs.y);
+            v[i + 1] = from_f32<T>(y * cs.x + x * cs.y);
+            w = w + 2 == s.rot ? 0 : w + 2;
+          }
+        }
+        *reinterpret_cast<uint4*>(s.out + (tok0 + t) * s.o_st + (int64_t)(seg0 + r - t * nseg) * s.o_ss + (int64_t)k * 16) = raw[q];
+      }
+    }
+  }
 }
 
 struct RopeCacheArgs {
@@ -185,25 +227,23 @@ __device__ __forceinline__ uint8_t e4m3_of(float x) {
   return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
 
-// One block per (token, part): part 0 writes the token's cache row, parts 1.. rotate hpb heads of
-// q each.  Two parts never touch the same bytes, so q may be rotated in place.
+// One block per (token, part): part p rotates hpb heads of q, part 0 also writes the token's cache row.
+// Parts never touch the same bytes, so q may be rotated in place.
 template <bool FP8, bool VEC>
 __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCacheArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* tab = reinterpret_cast<float2*>(smem);
-  uint8_t* stage = smem + ((a.q.rot * 8 + 15) & ~15);
+  const int half = a.q.rot >> 1, pairs = a.q.blocks * half;
+  float2* turns = reinterpret_cast<float2*>(smem);
+  uint32_t* table = reinterpret_cast<uint32_t*>(smem + half * 8);
+  uint8_t* stage = smem + ((half * 8 + pairs * 4 + 15) & ~15);
   const int64_t tok = blockIdx.x;
   const int tid = threadIdx.x;
-  for (int i = tid; i < (a.q.rot >> 1); i += kRotThreads)
-    fill_table(tab, a.g, a.q.rot, position(a.g, tok), i);
-  if (blockIdx.y > 0) {
-    const int seg0 = ((int)blockIdx.y - 1) * a.hpb;
-    rotate_segments<__nv_bfloat16, VEC>(a.q, a.g.interleaved, tab, stage, tok, 1, seg0,
-                                        min(a.hpb, a.q.segs - seg0));
-    return;
-  }
-  const int64_t slot = __ldg(reinterpret_cast<const long long*>(a.slots) + tok);
-  if (slot < 0) return;  // padding token: nothing is cached
+  for (int i = tid; i < half; i += kRotThreads) turns[i] = turn_of(a.g, position(a.g, tok), i);
+  for (int j = tid; j < pairs; j += kRotThreads) table[j] = pair_entry(a.q, a.g.interleaved, j);
+  const int64_t slot = blockIdx.y == 0 ? __ldg(reinterpret_cast<const long long*>(a.slots) + tok) : -1;
+  const int seg0 = (int)blockIdx.y * a.hpb;
+  rotate_segments<__nv_bfloat16, VEC>(a.q, a.g.interleaved, table, turns, stage, tok, 1, seg0, min(a.hpb, a.q.segs - seg0));
+  if (slot < 0) return;  // a part without the row, or a padding token: nothing is cached
   if (slot >= a.num_slots) {
     if (tid == 0 && a.status) atomicOr(a.status, QMLA_DEV_ERR_INDEX);
     return;
@@ -239,8 +279,25 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
         reinterpret_cast<__nv_bfloat16*>(dst)[d] = v;
     }
   }
+  // rope keys, from the last threads down (the first have the latent): an FP8 row rounds the rotated
+  // value once, not to bf16 first
+  const int dist = a.g.interleaved ? 1 : half;
+  for (int j = kRotThreads - 1 - tid; j < pairs; j += kRotThreads) {
+    const uint32_t e = table[j];
+    const float2 cs = turns[e >> 16];
+    const int d = e & 0xffffu;
+    const float x = __bfloat162float(kp[d]), y = __bfloat162float(kp[d + dist]);
+    const float ra = x * cs.x - y * cs.y, rb = y * cs.x + x * cs.y;
+    if constexpr (FP8) {
+      dst[a.rank + d] = e4m3_of(ra * inv);
+      dst[a.rank + d + dist] = e4m3_of(rb * inv);
+    } else {
+      reinterpret_cast<__nv_bfloat16*>(dst)[a.rank + d] = __float2bfloat16_rn(ra);
+      reinterpret_cast<__nv_bfloat16*>(dst)[a.rank + d + dist] = __float2bfloat16_rn(rb);
+    }
+  }
   // score divisors: as they are (bf16), log2 codes, or raw bf16 bytes
-  for (int h = tid; h < a.heads; h += kRotThreads) {
+  for (int h = (tid + kRotThreads / 2) % kRotThreads; h < a.heads; h += kRotThreads) {
     const __nv_bfloat16 rb = kp[a.win + h];
     if constexpr (!FP8) {
       reinterpret_cast<__nv_bfloat16*>(dst)[a.rank + a.win + h] = rb;
@@ -254,18 +311,6 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
       dst[a.rank + a.win + 2 * h + 1] = (uint8_t)(bits >> 8);
     }
   }
-  __syncthreads();  // the sines
-  // rope keys: an FP8 row rounds the rotated value once (not to bf16 first)
-  for (int e = tid; e < a.win; e += kRotThreads) {
-    const int w = e % a.q.rot;
-    const float2 cs = tab[w];
-    const float y = __bfloat162float(kp[e]) * cs.x +
-                    __bfloat162float(kp[e - w + partner(w, a.q.rot, a.g.interleaved)]) * cs.y;
-    if constexpr (FP8)
-      dst[a.rank + e] = e4m3_of(y * inv);
-    else
-      reinterpret_cast<__nv_bfloat16*>(dst)[a.rank + e] = __float2bfloat16_rn(y);
-  }
 }
 
 bool aligned16(const void* p, int64_t s1, int64_t s2) {
@@ -278,11 +323,18 @@ int launch_rotary(const RotSpan& s, const RotAngles& g, int64_t n, bool vec, int
   const int64_t gx = (n + tpb - 1) / tpb;
   const int gy = (s.segs + spb - 1) / spb;
   if (gx > INT32_MAX || gy > 65535) return QMLA_E_UNSUPPORTED;
-  const size_t smem = ((size_t)tpb * s.rot * 8 + 15) / 16 * 16 + (size_t)tpb * spb * s.len * sizeof(T);
-  if (vec)
-    rotary_kernel<T, true><<<dim3((unsigned)gx, gy), kRotThreads, smem, st>>>(s, g, n, tpb, spb);
-  else
-    rotary_kernel<T, false><<<dim3((unsigned)gx, gy), kRotThreads, smem, st>>>(s, g, n, tpb, spb);
+  const dim3 grid((unsigned)gx, gy);
+  const int half = s.rot / 2;
+  const size_t head = ((size_t)tpb * half * 8 + (size_t)s.blocks * half * 4 + 15) / 16 * 16;
+  if (vec && g.interleaved && s.start % 2 == 0 && s.period % (16 / (int)sizeof(T)) == 0) {
+    rotary_pairs_kernel<T><<<grid, kRotThreads, head, st>>>(s, g, n, tpb, spb);
+  } else {
+    const size_t smem = head + (size_t)tpb * spb * s.len * sizeof(T);
+    if (vec)
+      rotary_kernel<T, true><<<grid, kRotThreads, smem, st>>>(s, g, n, tpb, spb);
+    else
+      rotary_kernel<T, false><<<grid, kRotThreads, smem, st>>>(s, g, n, tpb, spb);
+  }
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
 }
 
@@ -341,13 +393,14 @@ int qmla_rotary(const qmla_rotary_params* p, void* stream) {
     }
   }
   const RotAngles g{p->positions, p->positions_i64 != 0, p->steps, p->scale, p->interleaved != 0, p->adjoint != 0};
-  // A block takes about 8 KB (4 units per thread in flight), 2 KB when that leaves SMs idle:
+  // A block takes about 16 KB (4 units per thread in flight), 4 KB when that leaves SMs idle:
   // several heads of one token, or, where a whole token is less, several tokens.
   const int64_t seg_b = (int64_t)s.len * es;
-  int64_t target = 8192;
-  if (p->num_tokens * s.segs * seg_b < 2 * target * di.sms) target = 2048;
+  int64_t target = 16384;
+  if (p->num_tokens * s.segs * seg_b < 4 * target * di.sms) target = 4096;
   int spb = (int)std::max<int64_t>(1, std::min<int64_t>(s.segs, target / seg_b));
   int tpb = spb == s.segs ? (int)std::max<int64_t>(1, std::min<int64_t>(16, target / (seg_b * s.segs))) : 1;
+  tpb = std::max(1, std::min(tpb, 8192 / (s.rot * 4)));  // 8 KB of sines
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p->dtype == QMLA_DT_BF16) return launch_rotary<__nv_bfloat16>(s, g, p->num_tokens, vec, tpb, spb, st);
   if (p->dtype == QMLA_DT_F16) return launch_rotary<__half>(s, g, p->num_tokens, vec, tpb, spb, st);
@@ -411,11 +464,13 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) {
   a.status = p->status;
   a.vec_row = aligned16(a.latent, a.lat_st, 0) && aligned16(a.cache, a.page_b, a.tok_b) && p->rank % (fp8 ? 16 : 8) == 0;
   const bool vec = a.q.len * 2 % 16 == 0 && aligned16(a.q.x, a.q.x_st, a.q.x_ss) && aligned16(a.q.out, a.q.o_st, a.q.o_ss);
-  // q heads of a block: about 4 KB of them
-  a.hpb = std::max(1, std::min(p->num_heads, 4096 / (2 * a.q.len)));
-  const int parts = 1 + (p->num_heads + a.hpb - 1) / a.hpb;
+  // q heads of a block: about 16 KB of them, 4 KB when the tokens alone do not fill the SMs
+  const int64_t stage = p->num_tokens >= 2 * di.sms ? 16384 : 4096;
+  a.hpb = (int)std::max<int64_t>(1, std::min<int64_t>(p->num_heads, stage / (2 * a.q.len)));
+  const int parts = (p->num_heads + a.hpb - 1) / a.hpb;
   if (parts > 65535) return QMLA_E_UNSUPPORTED;
-  const size_t smem = ((size_t)a.q.rot * 8 + 15) / 16 * 16 + (size_t)a.hpb * a.q.len * 2;
+  const int half = a.q.rot / 2;
+  const size_t smem = ((size_t)half * 8 + (size_t)a.q.blocks * half * 4 + 15) / 16 * 16 + (size_t)a.hpb * a.q.len * 2;
   const dim3 grid((unsigned)p->num_tokens, parts);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (fp8)

@@ -527,10 +527,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     const bool two = !FP8 || a.rms_mode == 2;      // bytes per divisor
     const bool split = two && (m.skip & 1);        // raw bytes at an odd offset: a divisor may span two units
     const int items = kTile * (split ? a.heads : m.units);
-    auto factor = [&](uint32_t bits) -> float {
-      if (FP8 && a.rms_mode == 3) return gs * ex2_approx(3.0f - (float)bits * (6.0f / 255.0f));
-      const float rv = two ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits)) : e4m3_to_f32((uint8_t)bits) * kscale;
+    auto of_bf16 = [&](uint32_t bits) -> float {
+      const float rv = __uint_as_float(bits << 16);
       return rv > 0.f ? __fdividef(gs, rv) : gs;
+    };
+    auto of_e4m3 = [&](uint32_t bits) -> float {
+      const float rv = e4m3_to_f32((uint8_t)bits) * kscale;
+      return rv > 0.f ? __fdividef(gs, rv) : gs;
+    };
+    auto of_log8 = [&](uint32_t bits) -> float { return gs * ex2_approx(3.0f - (float)bits * (6.0f / 255.0f)); };
+    // the bytes of unit u -> the table's column t
+    auto unpack = [&](const uint32_t* w, int u, int t, auto of) {
+      const int h0 = 16 * u - m.skip;
+      float* col = fac + h0 * kTrFacPitch + t;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if ((unsigned)(h0 + e) < (unsigned)a.heads) col[e * kTrFacPitch] = of((w[e >> 2] >> (8 * (e & 3))) & 0xffu);
     };
     SegCursor cur{req0, lo, hi};
     int r, k0, k1, plo, phi;
@@ -585,19 +597,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
             if (split) {
               const uint8_t* p = row_of(k, t);
               if (p) p += m.base_b + m.skip + 2 * u;
-              fac[u * kTrFacPitch + t] = p ? factor((uint32_t)__ldg(p) | (uint32_t)__ldg(p + 1) << 8) : gs;
+              fac[u * kTrFacPitch + t] = p ? of_bf16((uint32_t)__ldg(p) | (uint32_t)__ldg(p + 1) << 8) : gs;
             } else if (two) {
               const int h0 = (16 * u - m.skip) / 2;
+              float* col = fac + h0 * kTrFacPitch + t;
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                if (h0 + e >= 0 && h0 + e < a.heads)
-                  fac[(h0 + e) * kTrFacPitch + t] = factor((w[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+                if ((unsigned)(h0 + e) < (unsigned)a.heads)
+                  col[e * kTrFacPitch] = of_bf16((w[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+            } else if (a.rms_mode == 3) {
+              unpack(w, u, t, of_log8);
             } else {
-              const int h0 = 16 * u - m.skip;
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (h0 + e >= 0 && h0 + e < a.heads)
-                  fac[(h0 + e) * kTrFacPitch + t] = factor((w[e >> 2] >> (8 * (e & 3))) & 0xffu);
+              unpack(w, u, t, of_e4m3);
             }
           }
         }
