@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import pathlib
+import struct
 
 _HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libqmla.so"
@@ -333,6 +334,20 @@ class EvictParams(ctypes.Structure):
     ]
 
 
+_FORMAT = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f"}
+
+
+def packer(cls) -> struct.Struct:
+    """Packs a call's parameters into the bytes of ``cls`` in one step (a null pointer is 0).
+
+    A ctypes structure of 30 fields takes several microseconds to fill, as long as the small
+    operators run; the functions that take one also take its bytes.
+    """
+    fmt = struct.Struct("@" + "".join(_FORMAT[t] for _, t in cls._fields_) + "0P")  # 0P: C's tail padding
+    assert fmt.size == ctypes.sizeof(cls)
+    return fmt
+
+
 # device status bits (qmla_read_status / the gather's status word)
 DEV_ERR_TIMEOUT, DEV_ERR_INDEX = 1, 2
 
@@ -360,14 +375,14 @@ PROTOTYPES = {
     "qmla_dcp_p2p_merge": (ctypes.c_int, [ctypes.POINTER(DcpP2PParams), _VP]),
     "qmla_dcp_read_status": (ctypes.c_int, [_VP, _VP, ctypes.POINTER(_I32)]),
     "qmla_gather_cache": (ctypes.c_int, [ctypes.POINTER(GatherParams), _VP]),
-    "qmla_tree_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(TreeParams), ctypes.POINTER(_I64)]),
-    "qmla_tree_attention": (ctypes.c_int, [ctypes.POINTER(TreeParams), _VP]),
-    "qmla_weights_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(WeightsParams), ctypes.POINTER(_I64)]),
-    "qmla_accumulate_weights": (ctypes.c_int, [ctypes.POINTER(WeightsParams), _VP]),
-    "qmla_evict_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(EvictParams), ctypes.POINTER(_I64)]),
-    "qmla_evict": (ctypes.c_int, [ctypes.POINTER(EvictParams), _VP]),
-    "qmla_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), _VP]),
-    "qmla_rope_cache_write": (ctypes.c_int, [ctypes.POINTER(RopeCacheParams), _VP]),
+    "qmla_tree_workspace_bytes": (ctypes.c_int, [_VP, ctypes.POINTER(_I64)]),
+    "qmla_tree_attention": (ctypes.c_int, [_VP, _VP]),
+    "qmla_weights_workspace_bytes": (ctypes.c_int, [_VP, ctypes.POINTER(_I64)]),
+    "qmla_accumulate_weights": (ctypes.c_int, [_VP, _VP]),
+    "qmla_evict_workspace_bytes": (ctypes.c_int, [_VP, ctypes.POINTER(_I64)]),
+    "qmla_evict": (ctypes.c_int, [_VP, _VP]),
+    "qmla_rotary": (ctypes.c_int, [_VP, _VP]),
+    "qmla_rope_cache_write": (ctypes.c_int, [_VP, _VP]),
 }
 
 _lib = None

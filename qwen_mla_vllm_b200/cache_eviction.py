@@ -7,13 +7,14 @@ and closes up its pages.  The plugin has no counterpart: its cache only grows
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .mla_decode_attention import _FP8_TYPES, _dt, rms_mode_for
-from .tree_attention import _workspace
+from .tree_attention import run_with_workspace
+
+_PACK_WEIGHTS = _lib.packer(_lib.WeightsParams)
+_PACK_EVICT = _lib.packer(_lib.EvictParams)
 
 
 def accumulate_attention_weights(q: torch.Tensor, kv_cache: torch.Tensor, weights: torch.Tensor, lse: torch.Tensor,
@@ -63,25 +64,15 @@ def accumulate_attention_weights(q: torch.Tensor, kv_cache: torch.Tensor, weight
     if reqs == 0 or heads == 0:
         return
     pe = q_pe if q_pe is not None else q
-    p = _lib.WeightsParams(
+    mode = rms_mode_for(kv_cache.dtype, rms_offset, rms_bf16, rms_log8)
+    run_with_workspace("qmla_accumulate_weights", _PACK_WEIGHTS.pack, (
         q.data_ptr(), q.stride(0), q.stride(1),
         pe.data_ptr() if q_pe is not None else q.data_ptr() + lat * q.element_size(), pe.stride(0), pe.stride(1),
         _dt(q), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), kv_cache.shape[0], width,
         _lib.DT_FP8E4M3 if fp8 else _lib.DT_BF16, page_size, block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], seq_lens.data_ptr(), reqs, qrows, heads, lat, qk, rms_offset,
-        rms_mode_for(kv_cache.dtype, rms_offset, rms_bf16, rms_log8), sm_scale, logit_cap or 0.0, decay,
-        k_scale.data_ptr() if k_scale is not None else None, lse.data_ptr(), lse.stride(0), weights.data_ptr(),
-        weights.stride(0), weights.shape[1], None, 0,
-        q.device.index if q.device.index is not None else torch.cuda.current_device())
-    lib = _lib.load()
-    need = ctypes.c_int64(0)
-    ref = ctypes.byref(p)
-    _lib.check("qmla_weights_workspace_bytes", lib.qmla_weights_workspace_bytes(ref, ctypes.byref(need)))
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    if need.value:
-        ws = workspace if workspace is not None else _workspace(q.device, stream, need.value)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    _lib.check("qmla_accumulate_weights", lib.qmla_accumulate_weights(ref, stream))
+        block_table.shape[1], seq_lens.data_ptr(), reqs, qrows, heads, lat, qk, rms_offset, mode, sm_scale,
+        logit_cap or 0.0, decay, k_scale.data_ptr() if k_scale is not None else 0, lse.data_ptr(), lse.stride(0),
+        weights.data_ptr(), weights.stride(0), weights.shape[1]), q.device, workspace)
 
 
 def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
@@ -138,19 +129,11 @@ def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
     if reqs == 0:
         return new_w, new_p, new_l
     es = kv_cache.element_size()
-    p = _lib.EvictParams(
+    run_with_workspace("qmla_evict", _PACK_EVICT.pack, (
         kv_cache.data_ptr(), kv_cache.stride(0) * es, kv_cache.stride(1) * es, kv_cache.shape[3] * es, kv_cache.shape[0],
         page_size, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], weights.data_ptr(),
         weights.stride(0), positions.data_ptr(), positions.stride(0), cols, seq_lens.data_ptr(),
-        budgets.data_ptr() if budgets is not None else None, min(budget, 2**31 - 1), sinks,
-        recent_from.data_ptr() if recent_from is not None else None, new_w.data_ptr(), new_p.data_ptr(), new_w.stride(0),
-        new_w.shape[1], new_l.data_ptr(), reqs, None, 0, dev.index if dev.index is not None else torch.cuda.current_device())
-    lib = _lib.load()
-    need = ctypes.c_int64(0)
-    ref = ctypes.byref(p)
-    _lib.check("qmla_evict_workspace_bytes", lib.qmla_evict_workspace_bytes(ref, ctypes.byref(need)))
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    ws = workspace if workspace is not None else _workspace(dev, stream, need.value)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    _lib.check("qmla_evict", lib.qmla_evict(ref, stream))
+        budgets.data_ptr() if budgets is not None else 0, min(budget, 2**31 - 1), sinks,
+        recent_from.data_ptr() if recent_from is not None else 0, new_w.data_ptr(), new_p.data_ptr(), new_w.stride(0),
+        new_w.shape[1], new_l.data_ptr(), reqs), dev, workspace)
     return new_w, new_p, new_l

@@ -73,29 +73,30 @@ __device__ __forceinline__ uint32_t key_of(const EvictArgs& a, int r, int64_t t,
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Exclusive sum over the block's warps (one value per warp, given by all its lanes) plus the sums
-// of the cluster's earlier CTAs; total = the cluster's sum.  box: 2 ints in shared memory.
-__device__ __forceinline__ int cluster_scan(cg::cluster_group& cl, int* warp_box, int* cta_box, int v) {
+// Exclusive sum over the cluster's warps of a value given by all lanes of each (two 32-bit sums side by
+// side in 64 bits).  cta_box: this scan's own place in shared memory, so that no barrier has to
+// follow before it is used again; the caller's next cluster barrier keeps it alive.
+__device__ __forceinline__ uint64_t cluster_scan(cg::cluster_group& cl, uint64_t* warp_box, uint64_t* cta_box, uint64_t v) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();  // warp_box is free
   if (lane == 0) warp_box[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    int x = warp_box[lane];
-    const int own = x;
+    uint64_t x = warp_box[lane];
+    const uint64_t own = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     warp_box[lane] = x - own;
     if (lane == 31) *cta_box = x;
   }
   cl.sync();
-  int base = 0;
-  for (int c = 0; c < (int)cl.block_rank(); ++c) base += *cl.map_shared_rank(cta_box, c);
-  base += warp_box[warp];
-  cl.sync();  // cta_box is read by all
+  uint64_t base = warp_box[warp];
+#pragma unroll
+  for (int c = 0; c < kMaxCluster; ++c)
+    if (c < (int)cl.block_rank()) base += *cl.map_shared_rank(cta_box, c);
   return base;
 }
 
@@ -105,8 +106,9 @@ __device__ __forceinline__ int cluster_scan(cg::cluster_group& cl, int* warp_box
 // A request's keys are read from memory once and stay in shared memory.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
   extern __shared__ __align__(16) uint32_t keys[];
-  __shared__ int hist[kBins];
-  __shared__ int warp_box[kSelWarps], cta_box;
+  __shared__ int hists[3][kBins];  // one per pass: none is cleared while the peers may still read it
+  __shared__ int warp_sum[kSelWarps];
+  __shared__ uint64_t warp_box[kSelWarps], cta_box[2];
   __shared__ int found_bin, found_above;
   cg::cluster_group cl = cg::this_cluster();
   const int C = cl.num_blocks(), rank = cl.block_rank();
@@ -130,8 +132,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
   const int64_t lo = n * rank / C, hi = n * (rank + 1) / C;
   const int m = (int)(hi - lo);
   auto key_at = [&](int i) { return a.keys_fit ? keys[i] : key_of(a, r, lo + i, recent); };
-  if (a.keys_fit)
+  if (a.keys_fit) {
+#pragma unroll 4
     for (int i = tid; i < m; i += kSelThreads) keys[i] = key_of(a, r, lo + i, recent);
+  }
+  for (int b = tid; b < 3 * kBins; b += kSelThreads) (&hists[0][0])[b] = 0;
+  __syncthreads();
   uint32_t prefix = 0;  // the bits of the K-th largest key found so far
   int64_t want = K;     // its rank among the keys that share them
   int shift = 32;
@@ -140,8 +146,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     const uint32_t above = pass == 0 ? 0u : 0xffffffffu << shift;  // bits that are fixed
     shift -= bits;
     const uint32_t mask = (1u << bits) - 1;
-    for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
-    __syncthreads();
+    int* hist = hists[pass];
+#pragma unroll 4
     for (int i = tid; i < m; i += kSelThreads) {
       const uint32_t k = key_at(i);
       if ((k & above) == prefix) atomicAdd(&hist[(k >> shift) & mask], 1);
@@ -150,10 +156,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     // the cluster's counts, bins taken from the top: thread t adds up the bins 2t and 2t + 1
     int c1 = 0, c0 = 0;
     const int b1 = kBins - 1 - 2 * tid, b0 = b1 - 1;
-    for (int c = 0; c < C; ++c) {
-      const int* h = cl.map_shared_rank(hist, c);
-      c1 += h[b1];
-      c0 += h[b0];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      if (c < C) {
+        const int2 h = *reinterpret_cast<const int2*>(cl.map_shared_rank(hist, c) + b0);
+        c1 += h.y;
+        c0 += h.x;
+      }
     }
     int x = c1 + c0;
     const int own = x;
@@ -162,20 +171,20 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) warp_box[warp] = x;
+    if (lane == 31) warp_sum[warp] = x;
     __syncthreads();
     if (warp == 0) {
-      int y = warp_box[lane];
+      int y = warp_sum[lane];
       const int o0 = y;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int z = __shfl_up_sync(0xffffffffu, y, o);
         if (lane >= o) y += z;
       }
-      warp_box[lane] = y - o0;
+      warp_sum[lane] = y - o0;
     }
     __syncthreads();
-    const int64_t before = warp_box[warp] + x - own;  // keys in higher bins
+    const int64_t before = warp_sum[warp] + x - own;  // keys in higher bins
     if (want > before && want <= before + c1) {
       found_bin = b1;
       found_above = (int)before;
@@ -183,7 +192,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
       found_bin = b0;
       found_above = (int)before + c1;
     }
-    cl.sync();  // the histograms are read by all before they are cleared
+    __syncthreads();
     prefix |= (uint32_t)found_bin << shift;
     want -= found_above;
     __syncthreads();
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     const bool is = i + lane < i1 && key_at(i + lane) == prefix;
     eq += __popc(__ballot_sync(0xffffffffu, is));
   }
-  const int eq0 = cluster_scan(cl, warp_box, &cta_box, eq);
+  const int eq0 = (int)cluster_scan(cl, warp_box, &cta_box[0], (uint64_t)eq);
   const unsigned below = (1u << lane) - 1;
   // of a run of 32 tokens: which stay (eq_seen counts the equal ones before it)
   auto stays = [&](int i, int& eq_seen) {
@@ -214,8 +223,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     movers += __popc(__ballot_sync(0xffffffffu, keep && t >= K));
     holes += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && !keep && t < K));
   }
-  int mv = cluster_scan(cl, warp_box, &cta_box, movers);
-  int ho = cluster_scan(cl, warp_box, &cta_box, holes);
+  const uint64_t at = cluster_scan(cl, warp_box, &cta_box[1], (uint64_t)movers << 32 | (uint32_t)holes);
+  int mv = (int)(at >> 32), ho = (int)(uint32_t)at;
   seen = eq0;
   for (int i = i0; i < i1; i += 32) {
     const bool keep = stays(i, seen);
@@ -233,6 +242,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
   }
   // the last warp of the last CTA has counted all movers
   if (rank == C - 1 && warp == kSelWarps - 1 && lane == 0) a.count[r] = mv;
+  cl.sync();  // no CTA leaves while a peer may still read its sums
 }
 
 constexpr int kMoveThreads = 256;

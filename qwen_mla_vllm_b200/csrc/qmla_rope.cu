@@ -45,6 +45,13 @@ __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v);
 template <>
 __device__ __forceinline__ float from_f32(float v) { return v; }
 
+// Quotients of small numbers by a launch constant: exact for n * d < 2^32.
+struct FastDiv {
+  uint32_t d, magic;
+  __host__ static FastDiv of(uint32_t d) { return FastDiv{d, d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u}; }
+  __device__ __forceinline__ int div(int n) const { return d > 1 ? (int)__umulhi((uint32_t)n, magic) : n; }
+};
+
 // One rotated span of a token: `segs` segments (heads) of `len` elements, each a run of
 // heads of `period` dims whose dims [start, start + blocks * rot) turn, rot at a time.
 struct RotSpan {
@@ -52,6 +59,7 @@ struct RotSpan {
   uint8_t* out;
   int64_t x_st, x_ss, o_st, o_ss;  // bytes per token, per segment
   int segs, len, period, start, rot, blocks;
+  FastDiv by_units, by_segs, by_half;  // units of a segment, segments of a block, pairs of a rotated block
 };
 
 struct RotAngles {
@@ -78,7 +86,7 @@ __device__ __forceinline__ float2 turn_of(const RotAngles& g, int64_t pos, int i
 
 // Window pair j -> (offset of its first element in a head, pair of its block).
 __device__ __forceinline__ uint32_t pair_entry(const RotSpan& s, int interleaved, int j) {
-  const int half = s.rot >> 1, blk = j / half, i = j - blk * half;
+  const int half = s.rot >> 1, blk = s.by_half.div(j), i = j - blk * half;
   return (uint32_t)(s.start + blk * s.rot + (interleaved ? 2 * i : i)) | (uint32_t)i << 16;
 }
 
@@ -96,8 +104,8 @@ __device__ __forceinline__ void rotate_segments(const RotSpan& s, int interleave
   const int total = ntok * nseg * ups;
 #pragma unroll 4
   for (int u = threadIdx.x; u < total; u += kRotThreads) {
-    const int r = u / ups, k = u - r * ups;
-    const int t = r / nseg, sg = r - t * nseg;
+    const int r = s.by_units.div(u), k = u - r * ups;
+    const int t = ntok == 1 ? 0 : s.by_segs.div(r), sg = r - t * nseg;
     const uint8_t* p = s.x + (tok0 + t) * s.x_st + (int64_t)(seg0 + sg) * s.x_ss + (int64_t)k * V * sizeof(T);
     if constexpr (VEC)
       reinterpret_cast<uint4*>(stage)[u] = *reinterpret_cast<const uint4*>(p);
@@ -124,8 +132,8 @@ __device__ __forceinline__ void rotate_segments(const RotSpan& s, int interleave
   __syncthreads();
 #pragma unroll 4
   for (int u = threadIdx.x; u < total; u += kRotThreads) {
-    const int r = u / ups, k = u - r * ups;
-    const int t = r / nseg, sg = r - t * nseg;
+    const int r = s.by_units.div(u), k = u - r * ups;
+    const int t = ntok == 1 ? 0 : s.by_segs.div(r), sg = r - t * nseg;
     uint8_t* p = s.out + (tok0 + t) * s.o_st + (int64_t)(seg0 + sg) * s.o_ss + (int64_t)k * V * sizeof(T);
     if constexpr (VEC)
       *reinterpret_cast<uint4*>(p) = reinterpret_cast<const uint4*>(stage)[u];
@@ -146,7 +154,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotSpan s, co
   const int ntok = (int)min((int64_t)tpb, n - tok0);
   const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
   for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
-    const int t = i / half, k = i - t * half;
+    const int t = s.by_half.div(i), k = i - t * half;
     turns[i] = turn_of(g, position(g, tok0 + t), k);
   }
   for (int j = threadIdx.x; j < pairs; j += kRotThreads) table[j] = pair_entry(s, g.interleaved, j);
@@ -166,30 +174,32 @@ __global__ void __launch_bounds__(kRotThreads) rotary_pairs_kernel(const RotSpan
   const int ntok = (int)min((int64_t)tpb, n - tok0);
   const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
   const int ups = s.len / V, total = ntok * nseg * ups;
-  for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
-    const int t = i / half, k = i - t * half;
-    turns[i] = turn_of(g, position(g, tok0 + t), k);
-  }
-  __syncthreads();
-  for (int u0 = threadIdx.x; u0 < total; u0 += U * kRotThreads) {
+  for (int u0 = threadIdx.x; u0 - (int)threadIdx.x < total; u0 += U * kRotThreads) {
     uint4 raw[U];
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int u = u0 + q * kRotThreads;
       if (u < total) {
-        const int r = u / ups, k = u - r * ups, t = r / nseg;
+        const int r = s.by_units.div(u), k = u - r * ups, t = ntok == 1 ? 0 : s.by_segs.div(r);
         raw[q] = *reinterpret_cast<const uint4*>(s.x + (tok0 + t) * s.x_st + (int64_t)(seg0 + r - t * nseg) * s.x_ss + (int64_t)k * 16);
       }
+    }
+    if (u0 == (int)threadIdx.x) {  // the sines, while the first units are on their way
+      for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
+        const int t = s.by_half.div(i), k = i - t * half;
+        turns[i] = turn_of(g, position(g, tok0 + t), k);
+      }
+      __syncthreads();
     }
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int u = u0 + q * kRotThreads;
       if (u < total) {
-        const int r = u / ups, k = u - r * ups, t = r / nseg;
+        const int r = s.by_units.div(u), k = u - r * ups, t = ntok == 1 ? 0 : s.by_segs.div(r);
         T* v = reinterpret_cast<T*>(&raw[q]);
         const float2* tb = turns + t * half;
         const int d0 = k * V - s.start;  // window dim of the unit's first element (even)
-        int w = d0 >= 0 ? d0 % s.rot : 0;
+        int w = d0 >= 0 && d0 < win ? d0 - 2 * half * s.by_half.div(d0 >> 1) : 0;
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
           if (d0 + i >= 0 && d0 + i < win) {
@@ -318,13 +328,16 @@ bool aligned16(const void* p, int64_t s1, int64_t s2) {
 }
 
 template <typename T>
-int launch_rotary(const RotSpan& s, const RotAngles& g, int64_t n, bool vec, int tpb, int spb,
+int launch_rotary(RotSpan s, const RotAngles& g, int64_t n, bool vec, int tpb, int spb,
                   cudaStream_t st) {
   const int64_t gx = (n + tpb - 1) / tpb;
   const int gy = (s.segs + spb - 1) / spb;
   if (gx > INT32_MAX || gy > 65535) return QMLA_E_UNSUPPORTED;
   const dim3 grid((unsigned)gx, gy);
   const int half = s.rot / 2;
+  s.by_units = FastDiv::of(s.len / (vec ? 16 / (int)sizeof(T) : 1));
+  s.by_segs = FastDiv::of(spb);
+  s.by_half = FastDiv::of(half);
   const size_t head = ((size_t)tpb * half * 8 + (size_t)s.blocks * half * 4 + 15) / 16 * 16;
   if (vec && g.interleaved && s.start % 2 == 0 && s.period % (16 / (int)sizeof(T)) == 0) {
     rotary_pairs_kernel<T><<<grid, kRotThreads, head, st>>>(s, g, n, tpb, spb);
@@ -470,6 +483,9 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) {
   const int parts = (p->num_heads + a.hpb - 1) / a.hpb;
   if (parts > 65535) return QMLA_E_UNSUPPORTED;
   const int half = a.q.rot / 2;
+  a.q.by_units = FastDiv::of(a.q.len / (vec ? 8 : 1));
+  a.q.by_segs = FastDiv::of(a.hpb);
+  a.q.by_half = FastDiv::of(half);
   const size_t smem = ((size_t)half * 8 + (size_t)a.q.blocks * half * 4 + 15) / 16 * 16 + (size_t)a.hpb * a.q.len * 2;
   const dim3 grid((unsigned)p->num_tokens, parts);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -11,16 +11,18 @@ million as at one, with no table of sines and nothing to rebuild when contexts g
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from . import _lib
 from .mla_gather import _status_word
+from .tree_attention import _raw_stream
 
 _DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
 _FP8 = (torch.float8_e4m3fn, torch.uint8)
+_PACK_ROTARY = _lib.packer(_lib.RotaryParams)
+_PACK_UPDATE = _lib.packer(_lib.RopeCacheParams)
 _RMS = {"native": _lib.RMS_NATIVE, "log8": _lib.RMS_LOG8, "bf16": _lib.RMS_BF16, "none": _lib.RMS_NONE}
 
 
@@ -134,12 +136,12 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor, 
         raise ValueError(f"dims [{start}, {start} + {blocks} * {rot}) lie outside a head of {dim}")
     if n == 0 or heads == 0:
         return out
-    p = _lib.RotaryParams(
+    idx = _index(x.device)
+    p = _PACK_ROTARY.pack(
         x.data_ptr(), x.stride(0), x.stride(1) if x.dim() == 3 else dim, out.data_ptr(), out.stride(0),
         out.stride(1) if x.dim() == 3 else dim, n, heads, dim, _DT[x.dtype], start, rot, blocks, interleaved, adjoint,
-        scale, positions.data_ptr(), positions.dtype == torch.int64, steps.data_ptr(), _index(x.device))
-    stream = torch.cuda.current_stream(x.device).cuda_stream
-    _lib.check("qmla_rotary", _lib.load().qmla_rotary(ctypes.byref(p), stream))
+        scale, positions.data_ptr(), positions.dtype == torch.int64, steps.data_ptr(), idx)
+    _lib.check("qmla_rotary", _lib.load().qmla_rotary(p, _raw_stream(idx)))
     return out
 
 
@@ -194,13 +196,13 @@ def rope_kv_cache_update(q_pe: torch.Tensor, k_pe: torch.Tensor, kv_c_normed: to
         raise TypeError("an FP8 cache needs k_scale, an fp32 scalar on the device")
     if n == 0 or q_pe.shape[1] == 0:
         return q_out
-    p = _lib.RopeCacheParams(
+    idx = _index(kv_cache.device)
+    p = _PACK_UPDATE.pack(
         q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
         kv_c_normed.data_ptr(), kv_c_normed.stride(0), k_pe.data_ptr(), k_pe.stride(0), positions.data_ptr(),
         slot_mapping.data_ptr(), steps.data_ptr(), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), n,
         kv_cache.shape[0], kv_cache.shape[1], width, _lib.DT_FP8E4M3 if fp8 else _lib.DT_BF16, q_pe.shape[1], rank,
         packed_rope, rot, local_heads, _RMS[rms_mode], interleaved, positions.dtype == torch.int64, scale,
-        k_scale.data_ptr() if fp8 else None, _status_word(kv_cache.device).data_ptr(), _index(kv_cache.device))
-    stream = torch.cuda.current_stream(kv_cache.device).cuda_stream
-    _lib.check("qmla_rope_cache_write", _lib.load().qmla_rope_cache_write(ctypes.byref(p), stream))
+        k_scale.data_ptr() if fp8 else 0, _status_word(kv_cache.device).data_ptr(), idx)
+    _lib.check("qmla_rope_cache_write", _lib.load().qmla_rope_cache_write(p, _raw_stream(idx)))
     return q_out

@@ -15,16 +15,36 @@ from . import _lib
 from .mla_decode_attention import _FP8_TYPES, _dt, rms_mode_for
 
 _ws: dict[tuple[int, int], torch.Tensor] = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> the current stream's handle
+_PACK = _lib.packer(_lib.TreeParams)
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Scratch of the calls on one stream of one device: kept, and grown when a call needs more."""
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
-    ws = _ws.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _ws[key] = ws
-    return ws
+def run_with_workspace(name: str, pack, args: tuple, device: torch.device, workspace: torch.Tensor | None) -> None:
+    """Call ``qmla_<name>`` on the current stream with ``args``, its workspace and the device.
+
+    Without a ``workspace``, scratch is kept for the stream (calls on two streams never share it) and
+    grown when the library asks for more; it refuses a small one before it launches anything.
+    """
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    stream = _raw_stream(idx)
+    lib = _lib.load()
+    ws = workspace if workspace is not None else _ws.get((idx, stream))
+    ptr, size = (ws.data_ptr(), ws.numel() * ws.element_size()) if ws is not None else (0, 0)
+    p = pack(*args, ptr, size, idx)
+    rc = getattr(lib, name)(p, stream)
+    if rc == _E_WORKSPACE and workspace is None:
+        need = ctypes.c_int64(0)
+        sizer = _SIZER[name]
+        _lib.check(sizer, getattr(lib, sizer)(p, ctypes.byref(need)))
+        ws = torch.empty(max(need.value, 1 << 20), dtype=torch.uint8, device=device)
+        _ws[(idx, stream)] = ws
+        rc = getattr(lib, name)(pack(*args, ws.data_ptr(), ws.numel(), idx), stream)
+    _lib.check(name, rc)
+
+
+_E_WORKSPACE = -4
+_SIZER = {"qmla_tree_attention": "qmla_tree_workspace_bytes", "qmla_accumulate_weights": "qmla_weights_workspace_bytes",
+          "qmla_evict": "qmla_evict_workspace_bytes"}
 
 
 def tree_masks(parents: torch.Tensor) -> torch.Tensor:
@@ -101,24 +121,14 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse
     if reqs * nodes == 0:
         return
     pe = q_pe if q_pe is not None else q
-    p = _lib.TreeParams(
+    mode = rms_mode_for(kv_cache.dtype, rms_offset, rms_bf16, rms_log8)
+    run_with_workspace("qmla_tree_attention", _PACK.pack, (
         q.data_ptr(), q.stride(0), q.stride(1),
         pe.data_ptr() if q_pe is not None else q.data_ptr() + rank * q.element_size(), pe.stride(0), pe.stride(1),
         _dt(q), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), kv_cache.shape[0], width,
         _lib.DT_FP8E4M3 if fp8 else _lib.DT_BF16, page_size, block_table.data_ptr(), block_table.stride(0),
         block_table.shape[1], ctx_lens.data_ptr(), tree_mask.data_ptr(),
-        tree_mask.stride(0) if tree_mask.dim() == 2 else 0, reqs, nodes, heads, rank, qk, rms_offset,
-        rms_mode_for(kv_cache.dtype, rms_offset, rms_bf16, rms_log8), sm_scale, logit_cap or 0.0,
-        k_scale.data_ptr() if k_scale is not None else None, o.data_ptr(), o.stride(0), o.stride(1), _dt(o),
-        lse.data_ptr() if lse is not None else None, lse.stride(0) if lse is not None else 0,
-        _dt(lse) if lse is not None else _lib.DT_F32, None, 0,
-        q.device.index if q.device.index is not None else torch.cuda.current_device())
-    lib = _lib.load()
-    need = ctypes.c_int64(0)
-    ref = ctypes.byref(p)
-    _lib.check("qmla_tree_workspace_bytes", lib.qmla_tree_workspace_bytes(ref, ctypes.byref(need)))
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    if need.value:
-        ws = workspace if workspace is not None else _workspace(q.device, stream, need.value)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    _lib.check("qmla_tree_attention", lib.qmla_tree_attention(ref, stream))
+        tree_mask.stride(0) if tree_mask.dim() == 2 else 0, reqs, nodes, heads, rank, qk, rms_offset, mode, sm_scale,
+        logit_cap or 0.0, k_scale.data_ptr() if k_scale is not None else 0, o.data_ptr(), o.stride(0), o.stride(1), _dt(o),
+        lse.data_ptr() if lse is not None else 0, lse.stride(0) if lse is not None else 0,
+        _dt(lse) if lse is not None else _lib.DT_F32), q.device, workspace)
