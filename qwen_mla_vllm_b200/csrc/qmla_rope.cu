@@ -90,57 +90,67 @@ __device__ __forceinline__ uint32_t pair_entry(const RotSpan& s, int interleaved
   return (uint32_t)(s.start + blk * s.rot + (interleaved ? 2 * i : i)) | (uint32_t)i << 16;
 }
 
-// Rotates segments [seg0, seg0 + nseg) of tokens [tok0, tok0 + ntok) by way of shared memory: loaded
-// and stored in whole 16-byte units (VEC) whatever the window's alignment (58 dims turn as halves of 29),
-// turned in place in between, a warp per head and a lane per pair.  Every element is staged before any
-// is written, so out may be x itself.  `table`: pair_entry of the window's pairs; `turns`: [ntok][rot / 2];
-// both are written before the call, the barrier below makes them visible.
+// Segments [seg0, seg0 + nseg) of tokens [tok0, tok0 + ntok) by way of shared memory: loaded and stored
+// in whole 16-byte units (VEC) whatever the window's alignment (58 dims turn as halves of 29), turned in
+// place in between, a warp per head and a lane per pair.  Every element is staged before any is
+// written, so out may be x itself.
 template <typename T, bool VEC>
-__device__ __forceinline__ void rotate_segments(const RotSpan& s, int interleaved, const uint32_t* table,
-                                                const float2* turns, uint8_t* stage, int64_t tok0, int ntok, int seg0,
-                                                int nseg) {
-  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-  const int ups = s.len / V;  // units per segment
-  const int total = ntok * nseg * ups;
-#pragma unroll 4
-  for (int u = threadIdx.x; u < total; u += kRotThreads) {
-    const int r = s.by_units.div(u), k = u - r * ups;
+struct Staged {
+  static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+  const RotSpan& s;
+  uint8_t* stage;
+  int64_t tok0;
+  int ntok, seg0, nseg;
+
+  __device__ __forceinline__ int total() const { return ntok * nseg * (s.len / V); }
+  __device__ __forceinline__ int64_t offset(int u, int64_t st, int64_t ss) const {
+    const int r = s.by_units.div(u), k = u - r * (s.len / V);
     const int t = ntok == 1 ? 0 : s.by_segs.div(r), sg = r - t * nseg;
-    const uint8_t* p = s.x + (tok0 + t) * s.x_st + (int64_t)(seg0 + sg) * s.x_ss + (int64_t)k * V * sizeof(T);
-    if constexpr (VEC)
-      reinterpret_cast<uint4*>(stage)[u] = *reinterpret_cast<const uint4*>(p);
-    else
-      reinterpret_cast<T*>(stage)[u] = *reinterpret_cast<const T*>(p);
+    return (tok0 + t) * st + (int64_t)(seg0 + sg) * ss + (int64_t)k * V * sizeof(T);
   }
-  __syncthreads();
-  const int half = s.rot >> 1, pairs = s.blocks * half;
-  const int per_tok = nseg * (s.len / s.period), rows = ntok * per_tok;  // heads
-  const int dist = interleaved ? 1 : half;
-  for (int row = threadIdx.x >> 5; row < rows; row += kRotWarps) {
-    T* head = reinterpret_cast<T*>(stage) + row * s.period;
-    const float2* tb = turns + (row / per_tok) * half;
-#pragma unroll 4
-    for (int j = threadIdx.x & 31; j < pairs; j += 32) {
-      const uint32_t e = table[j];
-      const float2 cs = tb[e >> 16];
-      T* pa = head + (e & 0xffffu);
-      const float x = to_f32(pa[0]), y = to_f32(pa[dist]);
-      pa[0] = from_f32<T>(x * cs.x - y * cs.y);
-      pa[dist] = from_f32<T>(y * cs.x + x * cs.y);
+  // starts the loads; what the caller does before turn() overlaps them
+  __device__ __forceinline__ void load() const {
+    const int n = total();
+    for (int u = threadIdx.x; u < n; u += kRotThreads) {
+      const uint8_t* p = s.x + offset(u, s.x_st, s.x_ss);
+      if constexpr (VEC)
+        cp_async_16(smem_u32(stage) + 16 * u, p, 16);
+      else
+        reinterpret_cast<T*>(stage)[u] = *reinterpret_cast<const T*>(p);
     }
   }
-  __syncthreads();
+  // table: pair_entry of the window's pairs; turns: [ntok][rot / 2]; both written by this block before
+  __device__ __forceinline__ void turn(int interleaved, const uint32_t* table, const float2* turns) const {
+    if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    const int half = s.rot >> 1, pairs = s.blocks * half;
+    const int per_tok = nseg * (s.len / s.period), rows = ntok * per_tok;  // heads
+    const int dist = interleaved ? 1 : half;
+    for (int row = threadIdx.x >> 5; row < rows; row += kRotWarps) {
+      T* head = reinterpret_cast<T*>(stage) + row * s.period;
+      const float2* tb = turns + (ntok == 1 ? 0 : row / per_tok) * half;
 #pragma unroll 4
-  for (int u = threadIdx.x; u < total; u += kRotThreads) {
-    const int r = s.by_units.div(u), k = u - r * ups;
-    const int t = ntok == 1 ? 0 : s.by_segs.div(r), sg = r - t * nseg;
-    uint8_t* p = s.out + (tok0 + t) * s.o_st + (int64_t)(seg0 + sg) * s.o_ss + (int64_t)k * V * sizeof(T);
-    if constexpr (VEC)
-      *reinterpret_cast<uint4*>(p) = reinterpret_cast<const uint4*>(stage)[u];
-    else
-      *reinterpret_cast<T*>(p) = reinterpret_cast<const T*>(stage)[u];
+      for (int j = threadIdx.x & 31; j < pairs; j += 32) {
+        const uint32_t e = table[j];
+        const float2 cs = tb[e >> 16];
+        T* pa = head + (e & 0xffffu);
+        const float x = to_f32(pa[0]), y = to_f32(pa[dist]);
+        pa[0] = from_f32<T>(x * cs.x - y * cs.y);
+        pa[dist] = from_f32<T>(y * cs.x + x * cs.y);
+      }
+    }
+    __syncthreads();
+    const int n = total();
+#pragma unroll 2
+    for (int u = threadIdx.x; u < n; u += kRotThreads) {
+      uint8_t* p = s.out + offset(u, s.o_st, s.o_ss);
+      if constexpr (VEC)
+        *reinterpret_cast<uint4*>(p) = reinterpret_cast<const uint4*>(stage)[u];
+      else
+        *reinterpret_cast<T*>(p) = reinterpret_cast<const T*>(stage)[u];
+    }
   }
-}
+};
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotSpan s, const RotAngles g,
@@ -153,12 +163,14 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotSpan s, co
   const int64_t tok0 = (int64_t)blockIdx.x * tpb;
   const int ntok = (int)min((int64_t)tpb, n - tok0);
   const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
+  const Staged<T, VEC> st{s, stage, tok0, ntok, seg0, nseg};
+  st.load();
   for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
     const int t = s.by_half.div(i), k = i - t * half;
     turns[i] = turn_of(g, position(g, tok0 + t), k);
   }
   for (int j = threadIdx.x; j < pairs; j += kRotThreads) table[j] = pair_entry(s, g.interleaved, j);
-  rotate_segments<T, VEC>(s, g.interleaved, table, turns, stage, tok0, ntok, seg0, nseg);
+  st.turn(g.interleaved, table, turns);
 }
 
 // Pairs side by side within 16-byte units: nothing is staged, a thread turns the units it loads, four
@@ -248,39 +260,60 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
   uint8_t* stage = smem + ((half * 8 + pairs * 4 + 15) & ~15);
   const int64_t tok = blockIdx.x;
   const int tid = threadIdx.x;
+  const int seg0 = (int)blockIdx.y * a.hpb;
+  const Staged<__nv_bfloat16, VEC> st{a.q, stage, tok, 1, seg0, min(a.hpb, a.q.segs - seg0)};
+  st.load();
+  // The row's own inputs, on their way during the rotation: a 16-byte unit of the latent for the first
+  // threads, a pair of rope keys and a divisor for the last ones.
+  const bool row = blockIdx.y == 0;
+  const int64_t slot = row ? __ldg(reinterpret_cast<const long long*>(a.slots) + tok) : -1;
+  const uint8_t* lat = a.latent + tok * a.lat_st;
+  const __nv_bfloat16* kp = reinterpret_cast<const __nv_bfloat16*>(a.k_pe + tok * a.kpe_st);
+  constexpr int kLatUnit = FP8 ? 2 : 1;  // 16-byte loads per 16-byte store
+  const int lat_units = a.vec_row ? a.rank / (FP8 ? 16 : 8) : 0;
+  const int dist = a.g.interleaved ? 1 : half, back = kRotThreads - 1 - tid;
+  uint4 lv[kLatUnit];
+  __nv_bfloat16 kx, ky, kr;
+  if (row) {
+    if (tid < lat_units)
+#pragma unroll
+      for (int i = 0; i < kLatUnit; ++i) lv[i] = __ldg(reinterpret_cast<const uint4*>(lat) + kLatUnit * tid + i);
+    if (back < pairs) {
+      const int d = pair_entry(a.q, a.g.interleaved, back) & 0xffffu;
+      kx = kp[d];
+      ky = kp[d + dist];
+    }
+    if (back < a.heads) kr = kp[a.win + back];
+  }
+  const float inv = FP8 && row ? 1.0f / __ldg(a.k_scale) : 1.0f;
   for (int i = tid; i < half; i += kRotThreads) turns[i] = turn_of(a.g, position(a.g, tok), i);
   for (int j = tid; j < pairs; j += kRotThreads) table[j] = pair_entry(a.q, a.g.interleaved, j);
-  const int64_t slot = blockIdx.y == 0 ? __ldg(reinterpret_cast<const long long*>(a.slots) + tok) : -1;
-  const int seg0 = (int)blockIdx.y * a.hpb;
-  rotate_segments<__nv_bfloat16, VEC>(a.q, a.g.interleaved, table, turns, stage, tok, 1, seg0, min(a.hpb, a.q.segs - seg0));
+  st.turn(a.g.interleaved, table, turns);
   if (slot < 0) return;  // a part without the row, or a padding token: nothing is cached
   if (slot >= a.num_slots) {
     if (tid == 0 && a.status) atomicOr(a.status, QMLA_DEV_ERR_INDEX);
     return;
   }
   uint8_t* dst = a.cache + slot / a.page_size * a.page_b + slot % a.page_size * a.tok_b;
-  const uint8_t* lat = a.latent + tok * a.lat_st;
-  const __nv_bfloat16* kp = reinterpret_cast<const __nv_bfloat16*>(a.k_pe + tok * a.kpe_st);
-  const float inv = FP8 ? 1.0f / __ldg(a.k_scale) : 1.0f;
   // latent: FP8 rows round x / k_scale once, saturating at +-448 (NaN stays NaN)
-  if (a.vec_row) {
-    if constexpr (FP8) {
-      for (int u = tid; u < a.rank / 16; u += kRotThreads) {
-        const uint4 v[2] = {reinterpret_cast<const uint4*>(lat)[2 * u], reinterpret_cast<const uint4*>(lat)[2 * u + 1]};
-        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(v);
-        alignas(16) __nv_fp8x2_storage_t w[8];
+  for (int u = tid; u < lat_units; u += kRotThreads) {
+    if (u != tid)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 f = __bfloat1622float2(b[i]);
-          w[i] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3);
-        }
-        reinterpret_cast<uint4*>(dst)[u] = *reinterpret_cast<const uint4*>(w);
+      for (int i = 0; i < kLatUnit; ++i) lv[i] = __ldg(reinterpret_cast<const uint4*>(lat) + kLatUnit * u + i);
+    if constexpr (FP8) {
+      const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(lv);
+      alignas(16) __nv_fp8x2_storage_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = __bfloat1622float2(b[i]);
+        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3);
       }
+      reinterpret_cast<uint4*>(dst)[u] = *reinterpret_cast<const uint4*>(w);
     } else {
-      for (int u = tid; u < a.rank / 8; u += kRotThreads)
-        reinterpret_cast<uint4*>(dst)[u] = reinterpret_cast<const uint4*>(lat)[u];
+      reinterpret_cast<uint4*>(dst)[u] = lv[0];
     }
-  } else {
+  }
+  if (!a.vec_row) {
     for (int d = tid; d < a.rank; d += kRotThreads) {
       const __nv_bfloat16 v = reinterpret_cast<const __nv_bfloat16*>(lat)[d];
       if constexpr (FP8)
@@ -289,14 +322,16 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
         reinterpret_cast<__nv_bfloat16*>(dst)[d] = v;
     }
   }
-  // rope keys, from the last threads down (the first have the latent): an FP8 row rounds the rotated
-  // value once, not to bf16 first
-  const int dist = a.g.interleaved ? 1 : half;
-  for (int j = kRotThreads - 1 - tid; j < pairs; j += kRotThreads) {
+  // rope keys: an FP8 row rounds the rotated value once, not to bf16 first
+  for (int j = back; j < pairs; j += kRotThreads) {
     const uint32_t e = table[j];
     const float2 cs = turns[e >> 16];
     const int d = e & 0xffffu;
-    const float x = __bfloat162float(kp[d]), y = __bfloat162float(kp[d + dist]);
+    if (j != back) {
+      kx = kp[d];
+      ky = kp[d + dist];
+    }
+    const float x = __bfloat162float(kx), y = __bfloat162float(ky);
     const float ra = x * cs.x - y * cs.y, rb = y * cs.x + x * cs.y;
     if constexpr (FP8) {
       dst[a.rank + d] = e4m3_of(ra * inv);
@@ -307,8 +342,8 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
     }
   }
   // score divisors: as they are (bf16), log2 codes, or raw bf16 bytes
-  for (int h = (tid + kRotThreads / 2) % kRotThreads; h < a.heads; h += kRotThreads) {
-    const __nv_bfloat16 rb = kp[a.win + h];
+  for (int h = back; h < a.heads; h += kRotThreads) {
+    const __nv_bfloat16 rb = h == back ? kr : kp[a.win + h];
     if constexpr (!FP8) {
       reinterpret_cast<__nv_bfloat16*>(dst)[a.rank + a.win + h] = rb;
     } else if (a.rms_mode == QMLA_RMS_LOG8) {

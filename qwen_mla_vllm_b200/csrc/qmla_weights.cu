@@ -11,11 +11,14 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstring>
+#include <type_traits>
 
 #include "qmla.h"
 #include "qmla_decode.cuh"
 #include "qmla_host.cuh"
+#include "qmla_pair.cuh"
 #include "qmla_qimage.cuh"
 
 using namespace qmla;
@@ -136,14 +139,15 @@ __global__ void __launch_bounds__(256) weights_generic_kernel(const WeightArgs a
 // tiles of all requests.  Per tile S^T[128 tokens, query rows] = K_tile . Q^T on tcgen05 (M = 128, a
 // token per TMEM lane), so a thread of the epilogue owns a token: it turns its S columns into
 // weights one after another and adds them in a register, with no exchange between threads and one
-// 4-byte store.  Warp 0 streams K by TMA boxes of up to `cps` 128-byte columns x 16 tokens, warp 1
-// issues the MMAs, warps 2-5 are the epilogue; S is double-buffered.
+// 4-byte store.  Warp 0 streams K by TMA boxes of up to `cps` 128-byte columns x 16 tokens (a second
+// load warp made no difference), warp 1 issues the MMAs, warps 2-5 and 6-9 are two epilogues for the even
+// and the odd tiles; S is double-buffered.
 // Bound: HBM, the QK columns and the rms tail of every cached token, once.  The kernel holds no
 // values, so what shared memory Q leaves is all K in flight.
 struct WeightMmaArgs {
   const int32_t* prefix;    // [reqs + 1] tiles
   const uint8_t* img;       // [reqs][img_bytes]
-  const float* meta;        // [reqs][3][np]: log2-domain lse (+inf: adds nothing), tokens seen, score scale
+  const float* meta;        // [reqs][3 np]: np pairs (score scale, log2-domain lse; +inf adds nothing), np tokens seen
   uint32_t img_bytes;
   int j0, jn;               // query rows j0 .. j0 + jn - 1 of every request in this pass; column h * jn + j
   int np;                   // columns rounded up to 16
@@ -160,7 +164,7 @@ struct WeightMaps {
   CUtensorMap wide;   // (element, token in group, column, group in page, page), box = cps columns x run
 };
 
-constexpr int kWThreads = 192;
+constexpr int kWThreads = 320;  // warp 0 loads, 1 multiplies, 2-5 and 6-9 are the epilogue groups
 constexpr int kWMaxRows = 128;
 constexpr int kWMaxUnits = 7;  // 96 bytes of divisors (48 heads x 2) plus the misalignment
 
@@ -178,9 +182,9 @@ __global__ void __launch_bounds__(256) weights_prep_kernel(const WeightArgs a, c
   if (lane == 0) {
     float* mt = meta + (int64_t)r * 3 * m.np;
     const float lse = live ? __ldg(a.lse + row * a.lse_sr + h) : INFINITY;
-    mt[col] = isfinite(lse) ? lse * kLog2e : INFINITY;
-    mt[m.np + col] = __int_as_float(live && isfinite(lse) ? __ldg(a.lens + row) : 0);
-    mt[2 * m.np + col] = inv * a.sm_scale * (FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f);
+    mt[2 * col] = inv * a.sm_scale * (FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f);
+    mt[2 * col + 1] = isfinite(lse) ? lse * kLog2e : INFINITY;
+    mt[2 * m.np + col] = __int_as_float(live ? __ldg(a.lens + row) : INT32_MAX);
   }
   if (blockIdx.x == 0 && blockIdx.y == 0) {  // exclusive prefix of the requests' tiles
     __shared__ int warp_sum[8];
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
     // ---------------- K boxes, and each request's Q image
@@ -287,22 +291,19 @@ __global__ void __launch_bounds__(kWThreads, 1)
         for (int s = 0; s < m.nslots && ok; ++s) {
           const int c0 = s * m.cps, nch = min(m.cps, m.chunks - c0);
           const bool plain = c0 + m.cps > m.full_chunks;
-          if (lane == 0) {
-            ok = mbar_wait(bar(b_kempty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
-            if (ok) mbar_expect_tx(bar(b_kfull + ring.idx), (uint32_t)nch * 16384u);
+          ok = mbar_wait(bar(b_kempty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(bar(b_kfull + ring.idx), (uint32_t)nch * 16384u);
+          const uint32_t slot = sbase + ring.idx * slot_bytes;
+          if (plain) {
+            if (c < nch)
+              tma_load_3d(slot + c * 16384 + b * m.run * 128, &maps.chunk, (c0 + c) * estep, y, mypg,
+                          bar(b_kfull + ring.idx), pol);
+          } else if (lane < nrun) {
+            tma_load_5d(slot + lane * m.run * m.cps * 128, &maps.wide, 0, 0, c0, y / 8, mypg, bar(b_kfull + ring.idx), pol);
           }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (ok) {
-            const uint32_t slot = sbase + ring.idx * slot_bytes;
-            if (plain) {
-              if (c < nch)
-                tma_load_3d(slot + c * 16384 + b * m.run * 128, &maps.chunk, (c0 + c) * estep, y, mypg,
-                            bar(b_kfull + ring.idx), pol);
-            } else if (lane < nrun) {
-              tma_load_5d(slot + lane * m.run * m.cps * 128, &maps.wide, 0, 0, c0, y / 8, mypg, bar(b_kfull + ring.idx), pol);
-            }
-            ++armed;
-          }
+          ++armed;
           ring.next(m.nk);
         }
       }
@@ -315,79 +316,82 @@ __global__ void __launch_bounds__(kWThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ---------------- S^T = K . Q^T
-    if (lane == 0) {
-      // formats: bf16 both; or e4m3 keys and the term's format for Q
-      const uint32_t idesc0 = make_idesc_f16(FP8 ? 0 : 1, 128, m.np, 0, 0);
-      const uint64_t q0 = make_sdesc(qbuf, 16, 1024, 2);
-      const uint32_t qc16 = (uint32_t)m.np * 128 >> 4, qt16 = (uint32_t)(m.chunks * m.np) * 128 >> 4;
-      SegCursor cur{req0, lo, hi};
-      int r, k0, k1, plo, phi;
-      uint32_t jt = 0, seg = 0;
-      Ring ring;
-      bool ok = true;
-      while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-        ok = mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status);
-        for (int k = k0; k < k1 && ok; ++k, ++jt) {
-          const uint32_t sb = jt & 1;
-          if (jt >= 2) ok = mbar_wait(bar(b_sempty + sb), ((jt - 2) >> 1) & 1, abort_flag, m.status);
+    // ---------------- S^T = K . Q^T, the whole warp issuing (qmla_pair.cuh)
+    const uint32_t q_lo = sdesc_lo(qbuf, 16);
+    const uint32_t qc16 = (uint32_t)m.np * 128 >> 4, qt16 = (uint32_t)(m.chunks * m.np) * 128 >> 4;
+    // formats: bf16 both; or e4m3 keys and the term's format for Q
+    const uint32_t idesc0 = make_idesc_f16(FP8 ? 0 : 1, 128, m.np, 0, 0);
+    SegCursor cur{req0, lo, hi};
+    int r, k0, k1, plo, phi;
+    uint32_t jt = 0, seg = 0;
+    Ring ring;
+    bool ok = true;
+    auto wait = [&](uint32_t b, uint32_t ph) {
+      ok = ok && mbar_wait(bar(b), ph, abort_flag, m.status);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
+      wait(b_qfull, seg & 1);
+      for (int k = k0; k < k1 && ok; ++k, ++jt) {
+        const uint32_t sb = jt & 1;
+        if (jt >= 2) wait(b_sempty + sb, ((jt - 2) >> 1) & 1);
+        tc_fence_after();
+        const uint32_t d = tmem + sb * m.np;
+        for (int s = 0; s < m.nslots; ++s) {
+          wait(b_kfull + ring.idx, ring.ph);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t d = tmem + sb * m.np;
-          for (int s = 0; s < m.nslots && ok; ++s) {
-            ok = mbar_wait(bar(b_kfull + ring.idx), ring.ph, abort_flag, m.status);
-            if (!ok) break;
-            tc_fence_after();
-            const int c0 = s * m.cps, nch = min(m.cps, m.chunks - c0);
-            const bool plain = c0 + m.cps > m.full_chunks;
-            const uint32_t slot = sbase + ring.idx * slot_bytes;
-            for (int ci = 0; ci < nch; ++ci) {
-              // column ci: plain slots keep its 128 rows together, wide ones every 8 rows
-              const uint64_t ad = plain ? make_sdesc(slot + ci * 16384, 16, 1024, 2)
-                                        : make_sdesc(slot + ci * 1024, 16, 1024 * m.cps, 2);
-              for (int t = 0; t < m.terms; ++t) {
-                const uint64_t bd = q0 + (uint64_t)(c0 + ci) * qc16 + (uint64_t)t * qt16;
-                const uint32_t idesc = idesc0 | (FP8 ? q_term_format(t) << 10 : 0u);
+          const int c0 = s * m.cps, nch = min(m.cps, m.chunks - c0);
+          // column ci: plain slots keep its 128 rows together, wide ones every 8 rows
+          const bool plain = c0 + m.cps > m.full_chunks;
+          const uint32_t a0 = sdesc_lo(sbase + ring.idx * slot_bytes, 16), a_hi = plain ? sdesc_hi(1024) : sdesc_hi(1024 * m.cps);
+          const uint32_t a_col = plain ? 16384 >> 4 : 1024 >> 4;
+          for (int ci = 0; ci < nch; ++ci) {
+            for (int t = 0; t < m.terms; ++t) {
+              const uint32_t al = a0 + ci * a_col, bl = q_lo + (uint32_t)(c0 + ci) * qc16 + (uint32_t)t * qt16;
+              const uint32_t idesc = idesc0 | (FP8 ? q_term_format(t) << 10 : 0u);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                  const uint32_t acc = (s | ci | t | ks) != 0;
-                  if constexpr (FP8)
-                    tc_mma_f8_ss(d, ad + ks * 2, bd + ks * 2, idesc, acc);
-                  else
-                    tc_mma_f16_ss(d, ad + ks * 2, bd + ks * 2, idesc, acc);
-                }
-              }
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma_warp<FP8>(d, al + ks * 2, a_hi, bl + ks * 2, sdesc_hi(1024), idesc, ks > 0 ? 1u : (uint32_t)(s | ci | t));
             }
-            tc_commit(bar(b_kempty + ring.idx));
-            ring.next(m.nk);
           }
-          if (ok) tc_commit(bar(b_sfull + sb));
+          tc_commit_warp(bar(b_kempty + ring.idx));
+          ring.next(m.nk);
         }
-        if (ok) tc_commit(bar(b_qempty));
-        ++seg;
+        if (ok) tc_commit_warp(bar(b_sfull + sb));
       }
-      volatile int never = 0;  // drain before TMEM is released
-      tc_commit(bar(b_fin));
-      mbar_wait(bar(b_fin), 0, &never, nullptr, 100000000ull);
+      if (ok) tc_commit_warp(bar(b_qempty));
+      ++seg;
     }
+    volatile int never = 0;  // drain before TMEM is released
+    __syncwarp();
+    tc_commit_warp(bar(b_fin));
+    mbar_wait(bar(b_fin), 0, &never, nullptr, 100000000ull);
     __syncwarp();
   } else {
-    // ---------------- weights: a token per thread
-    const int sp = warp & 3, tt = sp * 32 + lane;
-    const int et = threadIdx.x - 64;  // 0..127
+    // ---------------- weights: a token per thread, a group of four warps per tile
+    const int grp = (warp - 2) >> 2, sp = warp & 3, tt = sp * 32 + lane;
+    const int et = threadIdx.x - 64;  // 0..255
     const float kscale = FP8 && a.k_scale ? __ldg(a.k_scale) : 1.f;
     const int es = !FP8 || a.rms_mode == QMLA_RMS_BF16 ? 2 : 1;
-    const int rows = a.heads * m.jn;
     const bool cap = a.logit_cap > 0.f;
+    const float2* meta2 = reinterpret_cast<const float2*>(meta_s);
+    const float* lim_s = meta_s + 2 * m.np;
     SegCursor cur{req0, lo, hi};
     int r, k0, k1, plo, phi;
     uint32_t jt = 0;
     bool ok = true;  // a warp that gives up still takes the barriers of the segments left
     while (next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-      named_bar_sync(1, 128);  // the previous request's meta is no longer read
-      for (int i = et; i < 3 * m.np; i += 128) meta_s[i] = __ldg(m.meta + (int64_t)r * 3 * m.np + i);
-      named_bar_sync(1, 128);
+      named_bar_sync(1, 256);  // the previous request's meta is no longer read
+      for (int i = et; i < 3 * m.np; i += 256) meta_s[i] = __ldg(m.meta + (int64_t)r * 3 * m.np + i);
+      named_bar_sync(1, 256);
       const int64_t n = weight_len(a, r);
+      int shortest = INT32_MAX;  // tokens that every row sees
+      for (int c = lane; c < m.np; c += 32) shortest = min(shortest, __float_as_int(lim_s[c]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) shortest = min(shortest, __shfl_xor_sync(0xffffffffu, shortest, o));
       for (int k = k0; k < k1 && ok; ++k, ++jt) {
+        if ((int)(jt & 1) != grp) continue;
         const int64_t t = (int64_t)k * kTile + tt;
         // this token's divisors, on their way while the tile's S is computed
         alignas(16) uint8_t tail[16 * kWMaxUnits];
@@ -403,31 +407,57 @@ __global__ void __launch_bounds__(kWThreads, 1)
         }
         float* wp = a.w + r * a.w_sr + t;
         const float old = t < n ? *wp : 0.f;
-        const uint32_t sb = jt & 1;
-        ok = mbar_wait(bar(b_sfull + sb), (jt >> 1) & 1, abort_flag, m.status);
+        ok = mbar_wait(bar(b_sfull + grp), (jt >> 1) & 1, abort_flag, m.status);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        float sum = 0.f, f = 1.f;
-        int h = 0, j = 0;
-        for (int c0 = 0; c0 < rows; c0 += 16) {
-          float x[16];
-          tmem_ld16(tmem + ((uint32_t)(sp * 32) << 16) + sb * m.np + c0, x);
-          tmem_wait_ld();
+        auto factor = [&](int h) -> float {  // of head h (0 past the last: its column adds 2^-inf)
+          if (h >= a.heads) return 0.f;
+          if (m.units == 0 || !here) return 1.f;
+          const uint8_t* b = tail + m.skip + es * h;
+          return inv_rms_bits<FP8>(a.rms_mode, es == 1 ? *b : (uint32_t)b[0] | (uint32_t)b[1] << 8, kscale);
+        };
+        const uint32_t ta = tmem + ((uint32_t)(sp * 32) << 16) + grp * m.np;
+        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+        const bool all_seen = (int64_t)(k + 1) * kTile <= shortest && !cap;
+        // 16 columns at a time; column h * jn + j
+        auto columns = [&](auto jn_c) {
+          constexpr int JN = decltype(jn_c)::value;
+          for (int c0 = 0; c0 < m.np; c0 += 16) {
+            float x[16], f = 0.f;
+            tmem_ld16(ta + c0, x);
+            tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int c = c0 + i;
-            if (c < rows) {
-              if (j == 0 && m.units > 0 && here) {
-                const uint8_t* b = tail + m.skip + es * h;
-                f = inv_rms_bits<FP8>(a.rms_mode, es == 1 ? *b : (uint32_t)b[0] | (uint32_t)b[1] << 8, kscale);
-              }
-              float s = x[i] * (meta_s[2 * m.np + c] * f);
+            for (int i = 0; i < 16; ++i) {
+              if (i % JN == 0) f = factor(c0 / JN + i / JN);
+              const float2 mt = meta2[c0 + i];
+              s4[i & 3] += ex2_approx(x[i] * f * mt.x * kLog2e - mt.y);
+            }
+          }
+        };
+        if (all_seen && m.jn == 1) {
+          columns(std::integral_constant<int, 1>());
+        } else if (all_seen && m.jn == 2) {
+          columns(std::integral_constant<int, 2>());
+        } else if (all_seen && m.jn == 4) {
+          columns(std::integral_constant<int, 4>());
+        } else {
+          float f = 0.f;
+          int h = 0, j = 0;
+          for (int c0 = 0; c0 < m.np; c0 += 16) {
+            float x[16];
+            tmem_ld16(ta + c0, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (j == 0) f = factor(h);
+              const float2 mt = meta2[c0 + i];
+              float s = x[i] * f * mt.x;
               if (cap) s = a.logit_cap * tanhf(s / a.logit_cap);
-              const float e = ex2_approx(s * kLog2e - meta_s[c]);
-              if (t < __float_as_int(meta_s[m.np + c])) sum += e;
+              const float e = ex2_approx(s * kLog2e - mt.y);
+              if (t < __float_as_int(lim_s[c0 + i])) s4[i & 3] += e;
               if (++j == m.jn) {
                 j = 0;
                 ++h;
@@ -435,9 +465,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
             }
           }
         }
+        const float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(b_sempty + sb));
+        if (lane == 0) mbar_arrive(bar(b_sempty + grp));
         if (t < n) *wp = (m.first ? old * a.decay : old) + (here ? sum : 0.f);
       }
     }
