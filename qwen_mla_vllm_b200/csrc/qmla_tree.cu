@@ -442,7 +442,7 @@ int launch_tree_mma(const qmla_tree_params* p, const TreeArgs& a, const TreePlan
     tree_mma_kernel<FP8, T0><<<grid, kTrThreads, pl.smem, st>>>(maps, a, m);
   else
     tree_mma_kernel<FP8, T0 + 1><<<grid, kTrThreads, pl.smem, st>>>(maps, a, m);
-  tree_pieces_kernel<<<dim3(p->num_reqs, m.rows), 128, 0, st>>>(a, m);
+  tree_pieces_kernel<<<dim3(p->num_reqs, m.rows), p->rank / 4, 0, st>>>(a, m);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
 }
 

@@ -867,12 +867,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
 }
 
 // Joins the pieces of requests cut at range boundaries: o = sum_i 2^(lse_i - lse) o_i.  One block per
-// (request, query row).  Requests inside one range are final already.
-__global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, const TreeMma m) {
+// (request, query row), a thread per four dims, up to eight pieces' loads in flight.  Requests inside
+// one range are final already.
+__global__ void __launch_bounds__(192) tree_pieces_kernel(const TreeArgs a, const TreeMma m) {
   const int r = blockIdx.x, x = blockIdx.y;
   __shared__ int bnd[kMaxCtas + 1];
   const int plo = __ldg(m.prefix + r), phi = __ldg(m.prefix + r + 1);
-  for (int c = threadIdx.x; c <= m.ranges; c += 128) bnd[c] = __ldg(m.bounds + c);
+  for (int c = threadIdx.x; c <= m.ranges; c += blockDim.x) bnd[c] = __ldg(m.bounds + c);
   __syncthreads();
   auto range_of = [&](int t) {  // the non-empty range that holds tile t
     int lo = 0, hi = m.ranges;
@@ -939,18 +940,30 @@ __global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, cons
   const int np = np_s, node = x / a.heads, h = x - node * a.heads;
   const float inv = inv_s;
   uint8_t* op = a.o + (((int64_t)r * a.nodes + node) * a.o_sr + (int64_t)h * a.o_sh) * dt_size(a.o_dtype);
-  for (int d = threadIdx.x; d < a.rank; d += 128) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    int k = 0;
-    for (; k + 4 <= np; k += 4) {  // four loads in flight
+  const int d = 4 * threadIdx.x;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < np; k0 += 8) {
+    float4 v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = __ldg(m.part_o + at[k + e] * a.rank + d);
-        acc[e] += wts[k + e] == 0.f ? 0.f : wts[k + e] * v;
-      }
+    for (int e = 0; e < 8; ++e)
+      if (k0 + e < np) v[e] = __ldg(reinterpret_cast<const float4*>(m.part_o + at[k0 + e] * a.rank + d));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = k0 + e < np ? wts[k0 + e] : 0.f;
+      if (w == 0.f) continue;  // a piece without visible tokens holds nothing
+      acc.x += w * v[e].x;
+      acc.y += w * v[e].y;
+      acc.z += w * v[e].z;
+      acc.w += w * v[e].w;
     }
-    for (; k < np; ++k) acc[0] += wts[k] == 0.f ? 0.f : wts[k] * __ldg(m.part_o + at[k] * a.rank + d);
-    store_from_float(op + (int64_t)d * dt_size(a.o_dtype), a.o_dtype, ((acc[0] + acc[1]) + (acc[2] + acc[3])) * inv);
+  }
+  const float r4[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  if (a.o_dtype == 0 && m.o_vec) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(r4[0], r4[1]), hi = __floats2bfloat162_rn(r4[2], r4[3]);
+    *reinterpret_cast<uint2*>(op + (int64_t)d * 2) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_from_float(op + (int64_t)(d + e) * dt_size(a.o_dtype), a.o_dtype, r4[e]);
   }
 }
 
