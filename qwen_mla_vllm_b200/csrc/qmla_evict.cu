@@ -318,16 +318,18 @@ int make_evict_plan(const qmla_evict_params* p, EvictPlan* pl) {
 
 extern "C" {
 
-int qmla_evict_workspace_bytes(const qmla_evict_params* p, int64_t* bytes) {
+int qmla_evict_workspace_bytes(const qmla_evict_params* p, int64_t* bytes) try {
   if (!bytes) return QMLA_E_INVALID;
   EvictPlan pl;
   const int rc = make_evict_plan(p, &pl);
   if (rc != QMLA_OK) return rc;
   *bytes = pl.ws_total;
   return QMLA_OK;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
-int qmla_evict(const qmla_evict_params* p, void* stream) {
+int qmla_evict(const qmla_evict_params* p, void* stream) try {
   EvictPlan pl;
   const int rc = make_evict_plan(p, &pl);
   if (rc != QMLA_OK) return rc;
@@ -407,6 +409,8 @@ int qmla_evict(const qmla_evict_params* p, void* stream) {
     evict_move_kernel<<<dim3((unsigned)std::min(most, share), p->num_reqs), kMoveThreads, 0, st>>>(a);
   }
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
 }  // extern "C"

@@ -390,7 +390,7 @@ int launch_rotary(RotSpan s, const RotAngles& g, int64_t n, bool vec, int tpb, i
 
 extern "C" {
 
-int qmla_rotary(const qmla_rotary_params* p, void* stream) {
+int qmla_rotary(const qmla_rotary_params* p, void* stream) try {
   if (!p || p->num_tokens < 0 || p->num_heads <= 0 || p->head_dim <= 0 || p->start < 0 ||
       p->rot_dim < 2 || p->rot_dim % 2 != 0 || p->blocks < 1)
     return QMLA_E_INVALID;
@@ -453,9 +453,11 @@ int qmla_rotary(const qmla_rotary_params* p, void* stream) {
   if (p->dtype == QMLA_DT_BF16) return launch_rotary<__nv_bfloat16>(s, g, p->num_tokens, vec, tpb, spb, st);
   if (p->dtype == QMLA_DT_F16) return launch_rotary<__half>(s, g, p->num_tokens, vec, tpb, spb, st);
   return launch_rotary<float>(s, g, p->num_tokens, vec, tpb, spb, st);
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
-int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) {
+int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) try {
   if (!p || p->num_tokens < 0 || p->num_heads <= 0 || p->rank <= 0 || p->rope_width <= 0 ||
       p->rms_heads < 0 || p->rot_dim < 2 || p->rot_dim % 2 != 0 || p->rope_width % p->rot_dim != 0 ||
       p->page_size <= 0 || p->num_pages < 0)
@@ -531,6 +533,8 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) {
     vec ? rope_cache_kernel<false, true><<<grid, kRotThreads, smem, st>>>(a)
         : rope_cache_kernel<false, false><<<grid, kRotThreads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
 }  // extern "C"

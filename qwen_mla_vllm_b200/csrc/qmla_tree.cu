@@ -450,16 +450,18 @@ int launch_tree_mma(const qmla_tree_params* p, const TreeArgs& a, const TreePlan
 
 extern "C" {
 
-int qmla_tree_workspace_bytes(const qmla_tree_params* p, int64_t* bytes) {
+int qmla_tree_workspace_bytes(const qmla_tree_params* p, int64_t* bytes) try {
   if (!bytes) return QMLA_E_INVALID;
   TreePlan pl;
   const int rc = make_tree_plan(p, &pl);
   if (rc != QMLA_OK) return rc;
   *bytes = pl.ws_total;
   return QMLA_OK;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
-int qmla_tree_attention(const qmla_tree_params* p, void* stream) {
+int qmla_tree_attention(const qmla_tree_params* p, void* stream) try {
   TreePlan pl;
   int rc = make_tree_plan(p, &pl);
   if (rc != QMLA_OK) return rc;
@@ -522,6 +524,8 @@ int qmla_tree_attention(const qmla_tree_params* p, void* stream) {
   if (rc != QMLA_OK) return rc;
   if (a.nsplit > 1) tree_join_kernel<<<a.reqs * a.nodes * a.heads, 128, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
 }  // extern "C"

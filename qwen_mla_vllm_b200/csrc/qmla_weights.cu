@@ -615,7 +615,7 @@ int launch_mma(const qmla_weights_params* p, const WeightArgs& a, const WeightPl
 
 extern "C" {
 
-int qmla_weights_workspace_bytes(const qmla_weights_params* p, int64_t* bytes) {
+int qmla_weights_workspace_bytes(const qmla_weights_params* p, int64_t* bytes) try {
   if (!bytes) return QMLA_E_INVALID;
   const int rc = check_params(p);
   if (rc != QMLA_OK) return rc;
@@ -625,9 +625,11 @@ int qmla_weights_workspace_bytes(const qmla_weights_params* p, int64_t* bytes) {
   plan_mma(p, di, &pl);
   *bytes = pl.ws_total;
   return QMLA_OK;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
-int qmla_accumulate_weights(const qmla_weights_params* p, void* stream) {
+int qmla_accumulate_weights(const qmla_weights_params* p, void* stream) try {
   int rc = check_params(p);
   if (rc != QMLA_OK) return rc;
   if (p->num_reqs == 0) return QMLA_OK;
@@ -689,6 +691,8 @@ int qmla_accumulate_weights(const qmla_weights_params* p, void* stream) {
   else
     weights_generic_kernel<false><<<grid, 256, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
 }
 
 }  // extern "C"

@@ -1,12 +1,13 @@
 """``torch.library`` custom ops over libqmla: ``torch.ops.qmla.mla_decode``, ``gather_cache``,
-``rotary`` and ``rope_kv_cache_update``.
+``rotary``, ``rope_kv_cache_update``, ``tree_attention``, ``accumulate_attention_weights`` and
+``evict_cache``.
 
 vLLM compiles its model with torch.compile and captures CUDA graphs around it. A ctypes call
 inside a compiled region would break the graph. These ops are opaque to the compiler: each
 declares which arguments it writes (``o`` / ``lse``, ``dst``) and has a fake kernel that does
 nothing, so tracing never touches the library. The real kernels run the same entry points as
 ``mla_decode_attention.decode_attention_fwd``, ``mla_gather.gather_cache_torch`` and the functions
-of ``rotary``.
+of ``rotary``, ``tree_attention`` and ``cache_eviction``.
 
     qmla::mla_decode(Tensor q, Tensor kv_cache, Tensor(a!) o, Tensor(b!) lse, Tensor block_table,
                      Tensor seq_lens, Tensor workspace, int rank, int qk_dim, int rms_offset,
@@ -21,6 +22,15 @@ of ``rotary``.
                  Tensor slot_mapping, Tensor steps, Tensor(a!) kv_cache, Tensor(b!) q_out,
                  int packed_rope, int local_heads, bool interleaved, float scale, Tensor? k_scale,
                  str rms_mode) -> ()
+    qmla::tree_attention(Tensor q, Tensor kv_cache, Tensor(a!) o, Tensor(b!) lse, Tensor block_table,
+                 Tensor ctx_lens, Tensor tree_mask, int rank, float sm_scale, int page_size,
+                 int rms_offset, bool rms_bf16, bool rms_log8, float logit_cap, Tensor? k_scale) -> ()
+    qmla::accumulate_attention_weights(Tensor q, Tensor kv_cache, Tensor(a!) weights, Tensor lse,
+                 Tensor block_table, Tensor seq_lens, float sm_scale, int page_size, int rms_offset,
+                 bool rms_bf16, bool rms_log8, float logit_cap, Tensor? k_scale, int qrows, float decay) -> ()
+    qmla::evict_cache(Tensor(a!) kv_cache, Tensor weights, Tensor positions, Tensor block_table,
+                 Tensor seq_lens, Tensor(b!) new_weights, Tensor(c!) new_positions, Tensor(d!) new_lens,
+                 int budget, int page_size, int sinks, Tensor? recent_from) -> ()
 
 ``rms_mode`` of mla_decode is a ``QMLA_RMS_*`` code (0 none, 1 native, 2 bf16 bytes, 3 log8).
 Set ``rms_offset`` < 0 in gather_cache for a 2-byte cache (no rms layout).
@@ -31,10 +41,13 @@ from typing import Optional
 
 import torch
 
+from .cache_eviction import accumulate_attention_weights as _accumulate_attention_weights
+from .cache_eviction import evict_cache as _evict_cache
 from .mla_decode_attention import build_params, run_params
 from .mla_gather import gather_cache_torch
 from .rotary import rope_kv_cache_update as _rope_kv_cache_update
 from .rotary import rotary_embed
+from .tree_attention import tree_attention as _tree_attention
 
 
 @torch.library.custom_op("qmla::mla_decode", mutates_args=("o", "lse"), device_types="cuda")
@@ -118,4 +131,54 @@ def rope_kv_cache_update(q_pe: torch.Tensor, k_pe: torch.Tensor, kv_c_normed: to
 @rope_kv_cache_update.register_fake
 def _rope_kv_cache_update_fake(q_pe, k_pe, kv_c_normed, positions, slot_mapping, steps, kv_cache, q_out, packed_rope,
                                local_heads, interleaved, scale, k_scale, rms_mode) -> None:
+    return None
+
+
+@torch.library.custom_op("qmla::tree_attention", mutates_args=("o", "lse"), device_types="cuda")
+def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                   block_table: torch.Tensor, ctx_lens: torch.Tensor, tree_mask: torch.Tensor, rank: int,
+                   sm_scale: float, page_size: int, rms_offset: int, rms_bf16: bool, rms_log8: bool,
+                   logit_cap: float, k_scale: Optional[torch.Tensor]) -> None:
+    """Attention of a drafted token tree into ``o`` / ``lse`` (``qmla_tree_attention``)."""
+    _tree_attention(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, rank=rank, sm_scale=sm_scale,
+                    page_size=page_size, rms_offset=rms_offset, rms_bf16=rms_bf16, rms_log8=rms_log8,
+                    logit_cap=logit_cap, k_scale=k_scale)
+
+
+@tree_attention.register_fake
+def _tree_attention_fake(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, rank, sm_scale, page_size, rms_offset,
+                         rms_bf16, rms_log8, logit_cap, k_scale) -> None:
+    return None
+
+
+@torch.library.custom_op("qmla::accumulate_attention_weights", mutates_args=("weights",), device_types="cuda")
+def accumulate_attention_weights(q: torch.Tensor, kv_cache: torch.Tensor, weights: torch.Tensor, lse: torch.Tensor,
+                                 block_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float, page_size: int,
+                                 rms_offset: int, rms_bf16: bool, rms_log8: bool, logit_cap: float,
+                                 k_scale: Optional[torch.Tensor], qrows: int, decay: float) -> None:
+    """A step's softmax weights added to ``weights`` (``qmla_accumulate_weights``)."""
+    _accumulate_attention_weights(q, kv_cache, weights, lse, block_table, seq_lens, sm_scale=sm_scale,
+                                  page_size=page_size, rms_offset=rms_offset, rms_bf16=rms_bf16, rms_log8=rms_log8,
+                                  logit_cap=logit_cap, k_scale=k_scale, qrows=qrows, decay=decay)
+
+
+@accumulate_attention_weights.register_fake
+def _accumulate_attention_weights_fake(q, kv_cache, weights, lse, block_table, seq_lens, sm_scale, page_size,
+                                       rms_offset, rms_bf16, rms_log8, logit_cap, k_scale, qrows, decay) -> None:
+    return None
+
+
+@torch.library.custom_op("qmla::evict_cache", mutates_args=("kv_cache", "new_weights", "new_positions", "new_lens"),
+                         device_types="cuda")
+def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, new_weights: torch.Tensor, new_positions: torch.Tensor, new_lens: torch.Tensor,
+                budget: int, page_size: int, sinks: int, recent_from: Optional[torch.Tensor]) -> None:
+    """Keep each request's heaviest tokens and close up its pages (``qmla_evict``)."""
+    _evict_cache(kv_cache, weights, positions, block_table, seq_lens, budget, page_size=page_size, sinks=sinks,
+                 recent_from=recent_from, out=(new_weights, new_positions, new_lens))
+
+
+@evict_cache.register_fake
+def _evict_cache_fake(kv_cache, weights, positions, block_table, seq_lens, new_weights, new_positions, new_lens, budget,
+                      page_size, sinks, recent_from) -> None:
     return None
