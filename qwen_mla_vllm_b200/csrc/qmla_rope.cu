@@ -6,8 +6,14 @@
 // (p * frequency in 32-bit floats is off by up to 2^-24 * p turns' worth: 0.016 rad at 262,144).
 // Its top 32 bits, taken as a signed fraction in [-1/2, 1/2), go to sincospif.
 //   (a, b) -> scale * (a cos - b sin, b cos + a sin)        the adjoint turns the other way
-// Both kernels are byte movers bound by HBM (2 or 3 flops per byte): every element is read once
-// and written once.  A block's sines are computed once for all the heads it rotates.
+// These kernels move bytes (2 or 3 flops per byte): every element is read once and written once, a
+// block's sines are computed once for all the heads it rotates, and a block walks up to four token groups
+// with the next one's bytes on their way.  Measured on a B200 (copy bandwidth 6.55 TB/s): 32,768 tokens'
+// worth of bf16 pairs side by side 106 us, 3.8 TB/s (one group per block: 128 us); 16,384 tokens into an
+// FP8 cache, queries in place, 117 us, 3.5 TB/s.  What is left is the turning itself: two-byte shared
+// loads and stores of pairs whose halves start at odd offsets, and blocks' phases that do not overlap.
+// Resident warps count most there: eight blocks of 256 threads (32 registers, a few spilled words in the
+// unaligned forms) 117 us, six 156, five 158, two (unbounded registers, four pairs in flight) 209.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -24,9 +30,12 @@ using namespace qmla;
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotBlocks = 8;  // of them resident on an SM
 constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kMaxRot = 512;            // dims of one rotated block
 constexpr int kStageBytes = 16 * 1024;  // one staged segment at most
+constexpr int kWalk = 4;  // token groups (or tokens) of a block in a long call
+constexpr int kBlockBytes = 12 * 1024;  // what a block stages at a time, where a segment is no larger
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -59,7 +68,8 @@ struct RotSpan {
   uint8_t* out;
   int64_t x_st, x_ss, o_st, o_ss;  // bytes per token, per segment
   int segs, len, period, start, rot, blocks;
-  FastDiv by_units, by_segs, by_half;  // units of a segment, segments of a block, pairs of a rotated block
+  // units of a segment, segments of a block, pairs and rotated blocks of a head, rotated blocks of a token
+  FastDiv by_units, by_segs, by_half, by_blocks, by_items;
 };
 
 struct RotAngles {
@@ -92,7 +102,7 @@ __device__ __forceinline__ uint32_t pair_entry(const RotSpan& s, int interleaved
 
 // Segments [seg0, seg0 + nseg) of tokens [tok0, tok0 + ntok) by way of shared memory: loaded and stored
 // in whole 16-byte units (VEC) whatever the window's alignment (58 dims turn as halves of 29), turned in
-// place in between, a warp per head and a lane per pair.  Every element is staged before any is
+// place in between.  Every element is staged before any is
 // written, so out may be x itself.
 template <typename T, bool VEC>
 struct Staged {
@@ -119,26 +129,62 @@ struct Staged {
         reinterpret_cast<T*>(stage)[u] = *reinterpret_cast<const T*>(p);
     }
   }
-  // table: pair_entry of the window's pairs; turns: [ntok][rot / 2]; both written by this block before
-  __device__ __forceinline__ void turn(int interleaved, const uint32_t* table, const float2* turns) const {
-    if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    const int half = s.rot >> 1, pairs = s.blocks * half;
-    const int per_tok = nseg * (s.len / s.period), rows = ntok * per_tok;  // heads
-    const int dist = interleaved ? 1 : half;
-    for (int row = threadIdx.x >> 5; row < rows; row += kRotWarps) {
-      T* head = reinterpret_cast<T*>(stage) + row * s.period;
-      const float2* tb = turns + (ntok == 1 ? 0 : row / per_tok) * half;
-#pragma unroll 4
-      for (int j = threadIdx.x & 31; j < pairs; j += 32) {
-        const uint32_t e = table[j];
-        const float2 cs = tb[e >> 16];
-        T* pa = head + (e & 0xffffu);
-        const float x = to_f32(pa[0]), y = to_f32(pa[dist]);
-        pa[0] = from_f32<T>(x * cs.x - y * cs.y);
-        pa[dist] = from_f32<T>(y * cs.x + x * cs.y);
+  // turns: [ntok][rot / 2], made visible with the staged elements by a barrier
+  __device__ __forceinline__ void turn(int interleaved, const float2* turns) const {
+    const bool even = ((s.start | s.period) & 1) == 0;
+    if (interleaved && even)
+      turn_as<2>(1, turns);
+    else if (!interleaved && even && (s.rot & 3) == 0)
+      turn_as<1>(s.rot >> 1, turns);
+    else
+      turn_as<0>(interleaved ? 1 : s.rot >> 1, turns);
+    store();
+  }
+  // A lane keeps its pairs (their sines in registers while the block holds one token) and walks the rotated
+  // blocks; where a block has fewer pairs than a warp has lanes, the warp takes several at a time.
+  // Form 0: a pair as two elements `dist` apart; 1: two neighbouring pairs, a word of each half; 2: a pair
+  // that is one word.
+  template <int FORM>
+  __device__ __forceinline__ void turn_as(int dist, const float2* turns) const {
+    constexpr int P = FORM == 1 ? 2 : 1;
+    struct alignas(2 * sizeof(T)) Word { T a, b; };
+    const int half = s.rot >> 1, lanes = half / P, lane = threadIdx.x & 31;
+    const int items = nseg * (s.len / s.period) * s.blocks, all = ntok * items;
+    const int share = lanes < 32 ? 32 / lanes : 1, sub = lanes < 32 ? lane / lanes : 0;
+    if (sub >= share) return;
+    for (int i = P * (lane - sub * lanes); i < half; i += 32 * P) {
+      float2 cs[P];
+#pragma unroll
+      for (int q = 0; q < P; ++q) cs[q] = turns[i + q];
+      T* base = reinterpret_cast<T*>(stage) + s.start + (dist == 1 ? 2 * i : i);
+      for (int m = (threadIdx.x >> 5) * share + sub; m < all; m += kRotWarps * share) {
+        const int row = s.by_blocks.div(m);
+        T* at = base + row * s.period + (m - row * s.blocks) * s.rot;
+        if (ntok > 1)
+#pragma unroll
+          for (int q = 0; q < P; ++q) cs[q] = turns[s.by_items.div(m) * half + i + q];
+        auto turned = [](float2 c, T& x, T& y) {
+          const float fx = to_f32(x), fy = to_f32(y);
+          x = from_f32<T>(fx * c.x - fy * c.y);
+          y = from_f32<T>(fy * c.x + fx * c.y);
+        };
+        if constexpr (FORM == 0) {
+          turned(cs[0], at[0], at[dist]);
+        } else if constexpr (FORM == 1) {
+          Word v = *reinterpret_cast<const Word*>(at), w = *reinterpret_cast<const Word*>(at + dist);
+          turned(cs[0], v.a, w.a);
+          turned(cs[P - 1], v.b, w.b);
+          *reinterpret_cast<Word*>(at) = v;
+          *reinterpret_cast<Word*>(at + dist) = w;
+        } else {
+          Word v = *reinterpret_cast<const Word*>(at);
+          turned(cs[0], v.a, v.b);
+          *reinterpret_cast<Word*>(at) = v;
+        }
       }
     }
+  }
+  __device__ __forceinline__ void store() const {
     __syncthreads();
     const int n = total();
 #pragma unroll 2
@@ -152,77 +198,118 @@ struct Staged {
   }
 };
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotSpan s, const RotAngles g,
-                                                             int64_t n, int tpb, int spb) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int half = s.rot >> 1, pairs = s.blocks * half;
-  float2* turns = reinterpret_cast<float2*>(smem);
-  uint32_t* table = reinterpret_cast<uint32_t*>(smem + tpb * half * 8);
-  uint8_t* stage = smem + ((tpb * half * 8 + pairs * 4 + 15) & ~15);
-  const int64_t tok0 = (int64_t)blockIdx.x * tpb;
-  const int ntok = (int)min((int64_t)tpb, n - tok0);
-  const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
-  const Staged<T, VEC> st{s, stage, tok0, ntok, seg0, nseg};
-  st.load();
-  for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
-    const int t = s.by_half.div(i), k = i - t * half;
-    turns[i] = turn_of(g, position(g, tok0 + t), k);
-  }
-  for (int j = threadIdx.x; j < pairs; j += kRotThreads) table[j] = pair_entry(s, g.interleaved, j);
-  st.turn(g.interleaved, table, turns);
+// Commits the copies started so far as one group / waits until at most `left` groups are in flight.
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int left>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(left) : "memory");
 }
 
-// Pairs side by side within 16-byte units: nothing is staged, a thread turns the units it loads, four
-// in flight.
+// A block walks the token groups from its own on, gridDim.x apart, the next group's elements on their
+// way to the other half of the stage while it turns this one's.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRotThreads, kRotBlocks) rotary_kernel(const RotSpan s, const RotAngles g,
+                                                             int64_t n, int tpb, int spb) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int half = s.rot >> 1;
+  float2* turns = reinterpret_cast<float2*>(smem);
+  uint8_t* stage0 = smem + ((tpb * half * 8 + 15) & ~15);
+  const int stage_bytes = (tpb * spb * s.len * (int)sizeof(T) + 15) & ~15;
+  const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
+  const int64_t groups = (n + tpb - 1) / tpb;
+  auto group = [&](int64_t i, int buf) {
+    return Staged<T, VEC>{s, stage0 + buf * stage_bytes, i * tpb, (int)min((int64_t)tpb, n - i * tpb), seg0, nseg};
+  };
+  group(blockIdx.x, 0).load();
+  copies_commit();
+  int buf = 0;
+  for (int64_t i = blockIdx.x; i < groups; i += gridDim.x, buf ^= 1) {
+    const Staged<T, VEC> st = group(i, buf);
+    if (i + gridDim.x < groups) group(i + gridDim.x, buf ^ 1).load();
+    copies_commit();
+    for (int x = threadIdx.x; x < st.ntok * half; x += kRotThreads) {
+      const int t = s.by_half.div(x), k = x - t * half;
+      turns[x] = turn_of(g, position(g, st.tok0 + t), k);
+    }
+    copies_wait<1>();
+    __syncthreads();
+    st.turn(g.interleaved, turns);
+    __syncthreads();  // the stage and the sines are free
+  }
+}
+
+// Pairs side by side within 16-byte units: a thread turns the units it loads, two at a time, the next two
+// (of the next token group at the end) on their way before these are turned.  Two units and six resident
+// blocks 106 us at the size above; four units and four blocks 111, two and eight (spilling) 123.
 template <typename T>
-__global__ void __launch_bounds__(kRotThreads) rotary_pairs_kernel(const RotSpan s, const RotAngles g,
+__global__ void __launch_bounds__(kRotThreads, 6) rotary_pairs_kernel(const RotSpan s, const RotAngles g,
                                                                    int64_t n, int tpb, int spb) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int V = 16 / (int)sizeof(T), U = 4;
+  constexpr int V = 16 / (int)sizeof(T), U = 2;
   float2* turns = reinterpret_cast<float2*>(smem);
-  const int half = s.rot >> 1, win = s.blocks * s.rot;
-  const int64_t tok0 = (int64_t)blockIdx.x * tpb;
-  const int ntok = (int)min((int64_t)tpb, n - tok0);
+  const int half = s.rot >> 1, win = s.blocks * s.rot, ups = s.len / V;
   const int seg0 = blockIdx.y * spb, nseg = min(spb, s.segs - seg0);
-  const int ups = s.len / V, total = ntok * nseg * ups;
-  for (int u0 = threadIdx.x; u0 - (int)threadIdx.x < total; u0 += U * kRotThreads) {
-    uint4 raw[U];
+  const int64_t groups = (n + tpb - 1) / tpb;
+  auto total_of = [&](int64_t i) { return (int)min((int64_t)tpb, n - i * tpb) * nseg * ups; };
+  // unit u of group i: its token in the group and its window dim, and its place
+  auto place = [&](int64_t i, int u, int& t, int& k) -> int64_t {
+    const int r = s.by_units.div(u);
+    k = u - r * ups;
+    t = tpb == 1 ? 0 : s.by_segs.div(r);
+    return seg0 + r - t * nseg;
+  };
+  uint4 raw[U];
+  auto load = [&](int64_t i, int u0) {
+    const int total = i < groups ? total_of(i) : 0;
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int u = u0 + q * kRotThreads;
       if (u < total) {
-        const int r = s.by_units.div(u), k = u - r * ups, t = ntok == 1 ? 0 : s.by_segs.div(r);
-        raw[q] = *reinterpret_cast<const uint4*>(s.x + (tok0 + t) * s.x_st + (int64_t)(seg0 + r - t * nseg) * s.x_ss + (int64_t)k * 16);
+        int t, k;
+        const int64_t sg = place(i, u, t, k);
+        raw[q] = __ldcs(reinterpret_cast<const uint4*>(s.x + (i * tpb + t) * s.x_st + sg * s.x_ss + (int64_t)k * 16));
       }
     }
-    if (u0 == (int)threadIdx.x) {  // the sines, while the first units are on their way
-      for (int i = threadIdx.x; i < ntok * half; i += kRotThreads) {
-        const int t = s.by_half.div(i), k = i - t * half;
-        turns[i] = turn_of(g, position(g, tok0 + t), k);
-      }
-      __syncthreads();
+  };
+  load(blockIdx.x, threadIdx.x);
+  for (int64_t i = blockIdx.x; i < groups; i += gridDim.x) {
+    const int total = total_of(i), ntok = (int)min((int64_t)tpb, n - i * tpb);
+    __syncthreads();  // the sines are free
+    for (int x = threadIdx.x; x < ntok * half; x += kRotThreads) {
+      const int t = s.by_half.div(x), k = x - t * half;
+      turns[x] = turn_of(g, position(g, i * tpb + t), k);
     }
+    __syncthreads();
+    for (int u0 = threadIdx.x; u0 - (int)threadIdx.x < total; u0 += U * kRotThreads) {
+      uint4 cur[U];
 #pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const int u = u0 + q * kRotThreads;
-      if (u < total) {
-        const int r = s.by_units.div(u), k = u - r * ups, t = ntok == 1 ? 0 : s.by_segs.div(r);
-        T* v = reinterpret_cast<T*>(&raw[q]);
-        const float2* tb = turns + t * half;
-        const int d0 = k * V - s.start;  // window dim of the unit's first element (even)
-        int w = d0 >= 0 && d0 < win ? d0 - 2 * half * s.by_half.div(d0 >> 1) : 0;
+      for (int q = 0; q < U; ++q) cur[q] = raw[q];
+      if (u0 - (int)threadIdx.x + U * kRotThreads < total)
+        load(i, u0 + U * kRotThreads);
+      else
+        load(i + gridDim.x, threadIdx.x);
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          if (d0 + i >= 0 && d0 + i < win) {
-            const float2 cs = tb[w >> 1];
-            const float x = to_f32(v[i]), y = to_f32(v[i + 1]);
-            v[i] = from_f32<T>(x * cs.x - y * cs.y);
-            v[i + 1] = from_f32<T>(y * cs.x + x * cs.y);
-            w = w + 2 == s.rot ? 0 : w + 2;
+      for (int q = 0; q < U; ++q) {
+        const int u = u0 + q * kRotThreads;
+        if (u < total) {
+          int t, k;
+          const int64_t sg = place(i, u, t, k);
+          T* v = reinterpret_cast<T*>(&cur[q]);
+          const float2* tb = turns + t * half;
+          const int d0 = k * V - s.start;  // window dim of the unit's first element (even)
+          int w = d0 >= 0 && d0 < win ? d0 - 2 * half * s.by_half.div(d0 >> 1) : 0;
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            if (d0 + e >= 0 && d0 + e < win) {
+              const float2 cs = tb[w >> 1];
+              const float x = to_f32(v[e]), y = to_f32(v[e + 1]);
+              v[e] = from_f32<T>(x * cs.x - y * cs.y);
+              v[e + 1] = from_f32<T>(y * cs.x + x * cs.y);
+              w = w + 2 == s.rot ? 0 : w + 2;
+            }
           }
+          *reinterpret_cast<uint4*>(s.out + (i * tpb + t) * s.o_st + sg * s.o_ss + (int64_t)k * 16) = cur[q];
         }
-        *reinterpret_cast<uint4*>(s.out + (tok0 + t) * s.o_st + (int64_t)(seg0 + r - t * nseg) * s.o_ss + (int64_t)k * 16) = raw[q];
       }
     }
   }
@@ -243,63 +330,38 @@ struct RopeCacheArgs {
   const float* k_scale;
   int* status;
   int hpb;  // heads per block
+  int row_blocks, q_blocks;  // blocks that write rows; blocks per part of q
+  int64_t n;
 };
 
 __device__ __forceinline__ uint8_t e4m3_of(float x) {
   return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
 
-// One block per (token, part): part p rotates hpb heads of q, part 0 also writes the token's cache row.
-// Parts never touch the same bytes, so q may be rotated in place.
-template <bool FP8, bool VEC>
-__global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCacheArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int half = a.q.rot >> 1, pairs = a.q.blocks * half;
-  float2* turns = reinterpret_cast<float2*>(smem);
-  uint32_t* table = reinterpret_cast<uint32_t*>(smem + half * 8);
-  uint8_t* stage = smem + ((half * 8 + pairs * 4 + 15) & ~15);
-  const int64_t tok = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int seg0 = (int)blockIdx.y * a.hpb;
-  const Staged<__nv_bfloat16, VEC> st{a.q, stage, tok, 1, seg0, min(a.hpb, a.q.segs - seg0)};
-  st.load();
-  // The row's own inputs, on their way during the rotation: a 16-byte unit of the latent for the first
-  // threads, a pair of rope keys and a divisor for the last ones.
-  const bool row = blockIdx.y == 0;
-  const int64_t slot = row ? __ldg(reinterpret_cast<const long long*>(a.slots) + tok) : -1;
+// A token's cache row, by one warp: latent, rotated keys, divisors.  An FP8 row rounds x / k_scale once,
+// saturating at +-448 (NaN stays NaN), its rotated keys not to bf16 first.
+template <bool FP8>
+__device__ __forceinline__ void write_row(const RopeCacheArgs& a, int64_t tok) {
+  const int lane = threadIdx.x & 31;
+  const int64_t slot = __ldg(reinterpret_cast<const long long*>(a.slots) + tok);
+  const int half = a.q.rot >> 1, pairs = a.q.blocks * half, dist = a.g.interleaved ? 1 : half;
   const uint8_t* lat = a.latent + tok * a.lat_st;
   const __nv_bfloat16* kp = reinterpret_cast<const __nv_bfloat16*>(a.k_pe + tok * a.kpe_st);
-  constexpr int kLatUnit = FP8 ? 2 : 1;  // 16-byte loads per 16-byte store
-  const int lat_units = a.vec_row ? a.rank / (FP8 ? 16 : 8) : 0;
-  const int dist = a.g.interleaved ? 1 : half, back = kRotThreads - 1 - tid;
-  uint4 lv[kLatUnit];
-  __nv_bfloat16 kx, ky, kr;
-  if (row) {
-    if (tid < lat_units)
-#pragma unroll
-      for (int i = 0; i < kLatUnit; ++i) lv[i] = __ldg(reinterpret_cast<const uint4*>(lat) + kLatUnit * tid + i);
-    if (back < pairs) {
-      const int d = pair_entry(a.q, a.g.interleaved, back) & 0xffffu;
-      kx = kp[d];
-      ky = kp[d + dist];
-    }
-    if (back < a.heads) kr = kp[a.win + back];
-  }
-  const float inv = FP8 && row ? 1.0f / __ldg(a.k_scale) : 1.0f;
-  for (int i = tid; i < half; i += kRotThreads) turns[i] = turn_of(a.g, position(a.g, tok), i);
-  for (int j = tid; j < pairs; j += kRotThreads) table[j] = pair_entry(a.q, a.g.interleaved, j);
-  st.turn(a.g.interleaved, table, turns);
-  if (slot < 0) return;  // a part without the row, or a padding token: nothing is cached
+  if (slot < 0) return;  // a padding token: nothing is cached
   if (slot >= a.num_slots) {
-    if (tid == 0 && a.status) atomicOr(a.status, QMLA_DEV_ERR_INDEX);
+    if (lane == 0 && a.status) atomicOr(a.status, QMLA_DEV_ERR_INDEX);
     return;
   }
+  const int64_t pos = position(a.g, tok);
+  const float inv = FP8 ? 1.0f / __ldg(a.k_scale) : 1.0f;
   uint8_t* dst = a.cache + slot / a.page_size * a.page_b + slot % a.page_size * a.tok_b;
-  // latent: FP8 rows round x / k_scale once, saturating at +-448 (NaN stays NaN)
-  for (int u = tid; u < lat_units; u += kRotThreads) {
-    if (u != tid)
+  constexpr int kLoads = FP8 ? 2 : 1;  // 16-byte loads per 16-byte store
+  const int units = a.vec_row ? a.rank / (FP8 ? 16 : 8) : 0;
+#pragma unroll 2
+  for (int u = lane; u < units; u += 32) {
+    uint4 lv[kLoads];
 #pragma unroll
-      for (int i = 0; i < kLatUnit; ++i) lv[i] = __ldg(reinterpret_cast<const uint4*>(lat) + kLatUnit * u + i);
+    for (int i = 0; i < kLoads; ++i) lv[i] = __ldg(reinterpret_cast<const uint4*>(lat) + kLoads * u + i);
     if constexpr (FP8) {
       const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(lv);
       alignas(16) __nv_fp8x2_storage_t w[8];
@@ -314,7 +376,7 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
     }
   }
   if (!a.vec_row) {
-    for (int d = tid; d < a.rank; d += kRotThreads) {
+    for (int d = lane; d < a.rank; d += 32) {
       const __nv_bfloat16 v = reinterpret_cast<const __nv_bfloat16*>(lat)[d];
       if constexpr (FP8)
         dst[d] = e4m3_of(__bfloat162float(v) * inv);
@@ -322,16 +384,12 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
         reinterpret_cast<__nv_bfloat16*>(dst)[d] = v;
     }
   }
-  // rope keys: an FP8 row rounds the rotated value once, not to bf16 first
-  for (int j = back; j < pairs; j += kRotThreads) {
-    const uint32_t e = table[j];
-    const float2 cs = turns[e >> 16];
+#pragma unroll 2
+  for (int j = lane; j < pairs; j += 32) {
+    const uint32_t e = pair_entry(a.q, a.g.interleaved, j);
     const int d = e & 0xffffu;
-    if (j != back) {
-      kx = kp[d];
-      ky = kp[d + dist];
-    }
-    const float x = __bfloat162float(kx), y = __bfloat162float(ky);
+    const float x = __bfloat162float(kp[d]), y = __bfloat162float(kp[d + dist]);
+    const float2 cs = turn_of(a.g, pos, e >> 16);
     const float ra = x * cs.x - y * cs.y, rb = y * cs.x + x * cs.y;
     if constexpr (FP8) {
       dst[a.rank + d] = e4m3_of(ra * inv);
@@ -342,8 +400,8 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
     }
   }
   // score divisors: as they are (bf16), log2 codes, or raw bf16 bytes
-  for (int h = back; h < a.heads; h += kRotThreads) {
-    const __nv_bfloat16 rb = h == back ? kr : kp[a.win + h];
+  for (int h = lane; h < a.heads; h += 32) {
+    const __nv_bfloat16 rb = kp[a.win + h];
     if constexpr (!FP8) {
       reinterpret_cast<__nv_bfloat16*>(dst)[a.rank + a.win + h] = rb;
     } else if (a.rms_mode == QMLA_RMS_LOG8) {
@@ -358,32 +416,81 @@ __global__ void __launch_bounds__(kRotThreads) rope_cache_kernel(const RopeCache
   }
 }
 
+// The first row_blocks blocks write the cache rows, a warp per token; the others rotate q, each one part
+// (hpb heads) of tokens q_blocks apart, the next token's heads on their way to the other half of the stage
+// while this one's are turned.  No two blocks touch the same bytes, so q may be rotated in place.
+template <bool FP8, bool VEC>
+__global__ void __launch_bounds__(kRotThreads, kRotBlocks) rope_cache_kernel(const RopeCacheArgs a) {
+  if ((int)blockIdx.x < a.row_blocks) {
+    const int64_t tok = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
+    if (tok < a.n) write_row<FP8>(a, tok);
+    return;
+  }
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int half = a.q.rot >> 1;
+  float2* turns = reinterpret_cast<float2*>(smem);
+  uint8_t* stage0 = smem + ((half * 8 + 15) & ~15);
+  const int stage_bytes = (a.hpb * a.q.len * 2 + 15) & ~15;
+  const int x = blockIdx.x - a.row_blocks, part = x / a.q_blocks;
+  const int seg0 = part * a.hpb;
+  auto token = [&](int64_t tok, int buf) {
+    return Staged<__nv_bfloat16, VEC>{a.q, stage0 + buf * stage_bytes, tok, 1, seg0, min(a.hpb, a.q.segs - seg0)};
+  };
+  int64_t tok = x - part * a.q_blocks;
+  token(tok, 0).load();
+  copies_commit();
+  for (int buf = 0; tok < a.n; tok += a.q_blocks, buf ^= 1) {
+    const Staged<__nv_bfloat16, VEC> st = token(tok, buf);
+    if (tok + a.q_blocks < a.n) token(tok + a.q_blocks, buf ^ 1).load();
+    copies_commit();
+    for (int i = threadIdx.x; i < half; i += kRotThreads) turns[i] = turn_of(a.g, position(a.g, tok), i);
+    copies_wait<1>();
+    __syncthreads();
+    st.turn(a.g.interleaved, turns);
+    __syncthreads();  // the stage and the sines are free
+  }
+}
+
+template <typename K>
+bool room_for(K kernel, size_t smem) {
+  return smem <= 48 * 1024 ||
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
+}
+
+// Blocks of a walk over `groups` of work, `parts` blocks side by side on each: up to kWalk groups per
+// block, fewer where that would leave less than 16 blocks per SM.
+int64_t walk_blocks(int64_t groups, int64_t parts, int sms) {
+  const int64_t walk = std::max<int64_t>(1, std::min<int64_t>(kWalk, groups * parts / (16 * (int64_t)sms)));
+  return (groups + walk - 1) / walk;
+}
+
 bool aligned16(const void* p, int64_t s1, int64_t s2) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s1 % 16 == 0 && s2 % 16 == 0;
 }
 
 template <typename T>
-int launch_rotary(RotSpan s, const RotAngles& g, int64_t n, bool vec, int tpb, int spb,
+int launch_rotary(RotSpan s, const RotAngles& g, int64_t n, bool vec, int tpb, int spb, int sms,
                   cudaStream_t st) {
   const int64_t gx = (n + tpb - 1) / tpb;
   const int gy = (s.segs + spb - 1) / spb;
   if (gx > INT32_MAX || gy > 65535) return QMLA_E_UNSUPPORTED;
-  const dim3 grid((unsigned)gx, gy);
   const int half = s.rot / 2;
   s.by_units = FastDiv::of(s.len / (vec ? 16 / (int)sizeof(T) : 1));
   s.by_segs = FastDiv::of(spb);
   s.by_half = FastDiv::of(half);
-  const size_t head = ((size_t)tpb * half * 8 + (size_t)s.blocks * half * 4 + 15) / 16 * 16;
-  if (vec && g.interleaved && s.start % 2 == 0 && s.period % (16 / (int)sizeof(T)) == 0) {
-    rotary_pairs_kernel<T><<<grid, kRotThreads, head, st>>>(s, g, n, tpb, spb);
-  } else {
-    const size_t smem = head + (size_t)tpb * spb * s.len * sizeof(T);
-    if (vec)
-      rotary_kernel<T, true><<<grid, kRotThreads, smem, st>>>(s, g, n, tpb, spb);
-    else
-      rotary_kernel<T, false><<<grid, kRotThreads, smem, st>>>(s, g, n, tpb, spb);
-  }
-  return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+  s.by_blocks = FastDiv::of(s.blocks);
+  s.by_items = FastDiv::of(spb * (s.len / s.period) * s.blocks);
+  const size_t head = ((size_t)tpb * half * 8 + 15) / 16 * 16;
+  const dim3 grid((unsigned)walk_blocks(gx, gy, sms), gy);
+  const size_t stage = 2 * (((size_t)tpb * spb * s.len * sizeof(T) + 15) / 16 * 16);
+  auto launch = [&](auto kernel, size_t smem) {
+    if (!room_for(kernel, smem)) return (int)QMLA_E_CUDA;
+    kernel<<<grid, kRotThreads, smem, st>>>(s, g, n, tpb, spb);
+    return cudaGetLastError() == cudaSuccess ? (int)QMLA_OK : (int)QMLA_E_CUDA;
+  };
+  if (vec && g.interleaved && s.start % 2 == 0 && s.period % (16 / (int)sizeof(T)) == 0)
+    return launch(rotary_pairs_kernel<T>, head);
+  return vec ? launch(rotary_kernel<T, true>, head + stage) : launch(rotary_kernel<T, false>, head + stage);
 }
 
 }  // namespace
@@ -441,18 +548,18 @@ int qmla_rotary(const qmla_rotary_params* p, void* stream) try {
     }
   }
   const RotAngles g{p->positions, p->positions_i64 != 0, p->steps, p->scale, p->interleaved != 0, p->adjoint != 0};
-  // A block takes about 16 KB (4 units per thread in flight), 4 KB when that leaves SMs idle:
+  // A block takes about 12 KB (3 units per thread in flight), 4 KB when that leaves SMs idle:
   // several heads of one token, or, where a whole token is less, several tokens.
   const int64_t seg_b = (int64_t)s.len * es;
-  int64_t target = 16384;
+  int64_t target = kBlockBytes;
   if (p->num_tokens * s.segs * seg_b < 4 * target * di.sms) target = 4096;
   int spb = (int)std::max<int64_t>(1, std::min<int64_t>(s.segs, target / seg_b));
   int tpb = spb == s.segs ? (int)std::max<int64_t>(1, std::min<int64_t>(16, target / (seg_b * s.segs))) : 1;
   tpb = std::max(1, std::min(tpb, 8192 / (s.rot * 4)));  // 8 KB of sines
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p->dtype == QMLA_DT_BF16) return launch_rotary<__nv_bfloat16>(s, g, p->num_tokens, vec, tpb, spb, st);
-  if (p->dtype == QMLA_DT_F16) return launch_rotary<__half>(s, g, p->num_tokens, vec, tpb, spb, st);
-  return launch_rotary<float>(s, g, p->num_tokens, vec, tpb, spb, st);
+  if (p->dtype == QMLA_DT_BF16) return launch_rotary<__nv_bfloat16>(s, g, p->num_tokens, vec, tpb, spb, di.sms, st);
+  if (p->dtype == QMLA_DT_F16) return launch_rotary<__half>(s, g, p->num_tokens, vec, tpb, spb, di.sms, st);
+  return launch_rotary<float>(s, g, p->num_tokens, vec, tpb, spb, di.sms, st);
 } catch (...) {  // no exception leaves a C entry
   return QMLA_E_CUDA;
 }
@@ -514,8 +621,8 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) try {
   a.status = p->status;
   a.vec_row = aligned16(a.latent, a.lat_st, 0) && aligned16(a.cache, a.page_b, a.tok_b) && p->rank % (fp8 ? 16 : 8) == 0;
   const bool vec = a.q.len * 2 % 16 == 0 && aligned16(a.q.x, a.q.x_st, a.q.x_ss) && aligned16(a.q.out, a.q.o_st, a.q.o_ss);
-  // q heads of a block: about 16 KB of them, 4 KB when the tokens alone do not fill the SMs
-  const int64_t stage = p->num_tokens >= 2 * di.sms ? 16384 : 4096;
+  // q heads of a block: about 12 KB of them, 4 KB when the tokens alone do not fill the SMs
+  const int64_t stage = p->num_tokens >= 2 * di.sms ? kBlockBytes : 4096;
   a.hpb = (int)std::max<int64_t>(1, std::min<int64_t>(p->num_heads, stage / (2 * a.q.len)));
   const int parts = (p->num_heads + a.hpb - 1) / a.hpb;
   if (parts > 65535) return QMLA_E_UNSUPPORTED;
@@ -523,16 +630,22 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) try {
   a.q.by_units = FastDiv::of(a.q.len / (vec ? 8 : 1));
   a.q.by_segs = FastDiv::of(a.hpb);
   a.q.by_half = FastDiv::of(half);
-  const size_t smem = ((size_t)half * 8 + (size_t)a.q.blocks * half * 4 + 15) / 16 * 16 + (size_t)a.hpb * a.q.len * 2;
-  const dim3 grid((unsigned)p->num_tokens, parts);
+  a.q.by_blocks = FastDiv::of(a.q.blocks);
+  a.q.by_items = FastDiv::of(1);  // a block holds one token
+  const size_t smem = ((size_t)half * 8 + 15) / 16 * 16 + 2 * (((size_t)a.hpb * a.q.len * 2 + 15) / 16 * 16);
+  a.n = p->num_tokens;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (fp8)
-    vec ? rope_cache_kernel<true, true><<<grid, kRotThreads, smem, st>>>(a)
-        : rope_cache_kernel<true, false><<<grid, kRotThreads, smem, st>>>(a);
-  else
-    vec ? rope_cache_kernel<false, true><<<grid, kRotThreads, smem, st>>>(a)
-        : rope_cache_kernel<false, false><<<grid, kRotThreads, smem, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
+  const int64_t rows = (a.n + kRotWarps - 1) / kRotWarps, walk = walk_blocks(a.n, parts, di.sms);
+  if (rows + walk * parts > INT32_MAX) return QMLA_E_UNSUPPORTED;
+  a.row_blocks = (int)rows;
+  a.q_blocks = (int)walk;
+  auto launch = [&](auto kernel) {
+    if (!room_for(kernel, smem)) return (int)QMLA_E_CUDA;
+    kernel<<<(unsigned)(rows + walk * parts), kRotThreads, smem, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? (int)QMLA_OK : (int)QMLA_E_CUDA;
+  };
+  if (fp8) return vec ? launch(rope_cache_kernel<true, true>) : launch(rope_cache_kernel<true, false>);
+  return vec ? launch(rope_cache_kernel<false, true>) : launch(rope_cache_kernel<false, false>);
 } catch (...) {  // no exception leaves a C entry
   return QMLA_E_CUDA;
 }

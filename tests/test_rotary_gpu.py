@@ -48,9 +48,9 @@ def expect(x, pos, steps, start, blocks, interleaved, adjoint=False, scale=1.0):
     return y, mag
 
 
-def check(got, y, mag, dtype):
+def check(got, y, mag, dtype, half_step=0.0):
     g = got.double().cpu().numpy()
-    tol = U[dtype] * np.abs(y) * 1.0001 + 1e-6 * mag
+    tol = U[dtype] * np.abs(y) * 1.0001 + 1e-6 * mag + half_step
     bad = np.abs(g - y) > tol
     assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.abs(g - y).max():.3e}"
 
@@ -330,3 +330,37 @@ def test_refusals(cuda_device):
                      (dict(kv_cache=cache[:, :, 0]), ValueError)):
         with pytest.raises(err):
             rope_kv_cache_update(**dict(ok, **bad))
+
+
+# Widest segments (two stages of 16 KB and the sines pass 48 KB of shared memory) and calls long enough
+# for a block to walk several token groups, the last one ragged.
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype,shape", [
+    (torch.float32, (3, 2, 4096, 512, 0, 8)), (torch.bfloat16, (2, 1, 8192, 512, 0, 16)),
+    (torch.bfloat16, (8193, 12, 58, 58, 0, 1)), (torch.bfloat16, (4099, 5, 234, 58, 2, 4)),
+    (torch.float16, (40001, 1, 64, 64, 0, 1)),
+])
+def test_rotary_wide_and_long(cuda_device, dtype, shape, interleaved):
+    n, heads, dim, rot, start, blocks = shape
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, heads, dim, generator=g).to(dtype).to(cuda_device)
+    pos = torch.randint(0, 1 << 20, (n,), generator=g)
+    steps, _ = rotary_steps(rot, 1e6, device=cuda_device)
+    y, mag = expect(x, pos, steps.cpu(), start, blocks, interleaved)
+    # two million values reach f16's subnormals, spaced 2^-24: there even the exact value rounds by 2^-25
+    check(rotary_embed(x, pos.to(cuda_device), steps, start=start, blocks=blocks, interleaved=interleaved), y, mag, dtype,
+          half_step=2.0**-25 if dtype == torch.float16 else 0.0)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("fp8,mode", [(False, "native"), (True, "log8")])
+def test_rope_update_long(cuda_device, fp8, mode, interleaved):
+    n, heads, rank, groups, page = 8199, 9, 256, 2, 64
+    t, _, cache, scale, win, _ = update_case(cuda_device, n, heads, rank, groups, fp8, mode, page)
+    steps, _ = rotary_steps(58, 1e6, device=cuda_device)
+    before = cache.clone()
+    q = rope_kv_cache_update(**t, steps=steps, kv_cache=cache, packed_rope=win, local_heads=heads,
+                             q_out=torch.empty_like(t["q_pe"]), interleaved=interleaved, k_scale=scale, rms_mode=mode)
+    y, mag = expect(t["q_pe"], t["positions"], steps.cpu(), 0, groups, interleaved)
+    check(q, y, mag, torch.bfloat16)
+    check_rows(t, before, cache, scale, win, rank, heads, mode, steps.cpu(), page, interleaved)
