@@ -32,7 +32,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
     ``scaling`` (None: the plain ``base ** (-2i / rot_dim)``) is one of
       {"type": "linear", "factor": f}   every frequency divided by f;
       {"type": "ntk", "factor": f}      the base raised so that the last pair is slowed by f;
-      {"type": "llama3", "factor": f, "low_freq_factor": a, "high_freq_factor": b,
+      {"type": "banded", "factor": f, "low_freq_factor": a, "high_freq_factor": b,
        "original_max_position": n}      pairs slower than n / a turns are divided by f, faster than
                                         n / b kept, those between blended linearly in turns;
       {"type": "yarn", "factor": f, "original_max_position": n, "beta_fast": 32, "beta_slow": 1,
@@ -56,7 +56,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
             raise ValueError("ntk scaling needs more than one pair")
         b = base * f ** (rot_dim / (rot_dim - 2.0))
         return [b ** (-2.0 * i / rot_dim) for i in range(half)], 1.0
-    if kind == "llama3":
+    if kind == "banded":
         n = float(scaling["original_max_position"])
         lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
         if hi <= lo:
@@ -81,7 +81,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
             out.append(w * ((1.0 - t) + t / f))
         att = scaling.get("attention_factor")
         return out, float(att) if att is not None else (0.1 * math.log(f) + 1.0 if f > 1 else 1.0)
-    raise ValueError(f"scaling type {kind!r}: expected linear, ntk, llama3 or yarn")
+    raise ValueError(f"scaling type {kind!r}: expected linear, ntk, banded or yarn")
 
 
 def rotary_steps(rot_dim: int, base: float = 10000.0, scaling: dict | None = None, *,

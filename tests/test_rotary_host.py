@@ -42,7 +42,7 @@ def test_scalings():
     assert s == 1.0 and all(a == b / 4 for a, b in zip(lin, plain))
     ntk, _ = rotary_frequencies(64, 1e4, {"type": "ntk", "factor": 8})
     assert ntk[0] == 1.0 and ntk[-1] == pytest.approx(plain[-1] / 8, rel=1e-12)
-    cfg = {"type": "llama3", "factor": 8, "low_freq_factor": 1, "high_freq_factor": 4, "original_max_position": 8192}
+    cfg = {"type": "banded", "factor": 8, "low_freq_factor": 1, "high_freq_factor": 4, "original_max_position": 8192}
     l3, _ = rotary_frequencies(64, 5e5, cfg)
     base, _ = rotary_frequencies(64, 5e5)
     for a, w in zip(l3, base):
@@ -63,7 +63,7 @@ def test_scalings():
 
 @pytest.mark.parametrize("rot,scaling", [(7, None), (0, None), (8, {"type": "what"}), (8, {"type": "linear", "factor": 0}),
                                          (2, {"type": "ntk", "factor": 2}),
-                                         (8, {"type": "llama3", "factor": 2, "original_max_position": 10,
+                                         (8, {"type": "banded", "factor": 2, "original_max_position": 10,
                                               "low_freq_factor": 4, "high_freq_factor": 4})])
 def test_bad_frequencies(rot, scaling):
     with pytest.raises(ValueError):
