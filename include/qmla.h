@@ -36,6 +36,12 @@
  *                        done by one kernel over NVLink peer memory instead of
  *                        NCCL; no counterpart in the reference, which refuses
  *                        DCP (qwen_mla/mla_impl.py:552).
+ * Operators next to that path, without a counterpart in the reference:
+ *   qmla_rotary, qmla_rope_cache_write   rotary positions; a step's queries rotated
+ *                        and its rows written in one launch
+ *   qmla_tree_attention  attention of a drafted token tree
+ *   qmla_accumulate_weights, qmla_evict   per-token attention weight and the
+ *                        eviction from the cache by it
  */
 #ifndef QMLA_H_
 #define QMLA_H_

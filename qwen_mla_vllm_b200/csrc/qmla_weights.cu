@@ -6,6 +6,12 @@
 // for the tokens t before the longest of the request's row lengths.  lse is what the decode of the
 // same queries returned, so nothing is normalised here: one pass over the keys, one number per
 // token out.  Rows whose lse is not finite (nothing visible) add nothing.
+//
+// The tensor-core form is one persistent CTA per SM over 128-token tiles: S^T[128 tokens, query rows] =
+// K . Q^T, so that a token is a TMEM lane and the sum over the rows stays inside a thread.  The keys cross
+// HBM once (2.2 GB at 64 requests of up to 32k tokens, bf16): 385-402 us, 5.4-5.7 TB/s, 83-87% of the copy
+// bandwidth; over an FP8 cache, 16 requests x 4 rows x 8192 tokens, 70 us: short tiles, where the exponentials
+// of 96 rows per token and the launch of two kernels are no longer hidden.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -1,7 +1,7 @@
 """Accumulated attention weights and eviction on the GPU, against 64-bit and exact restatements.
 
 Bounds of a weight: a score is off by at most 2^-19 of the sum of its terms' magnitudes (32-bit sums;
-FP8 queries in two e4m3 terms) plus a few roundings of s and lse (1e-6 of 1 + |s| + |lse|), and
+FP8 queries in two 8-bit terms) plus a few roundings of s and lse (1e-6 of 1 + |s| + |lse|), and
 exp turns that into a relative error of each term of the sum.  Eviction moves numbers: all of it is exact.
 """
 from __future__ import annotations

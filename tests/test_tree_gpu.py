@@ -1,7 +1,7 @@
 """Attention of a drafted token tree on the GPU against its 64-bit formula.
 
 Bounds (tree_util.tree_ref): scores are products accumulated in 32 bits (FP8 queries are split in two
-e4m3 terms that keep 2^-19 of the largest element), so a score is off by at most 2^-19 of the sum of
+8-bit terms that keep 2^-19 of the largest element), so a score is off by at most 2^-19 of the sum of
 its terms' magnitudes; each softmax weight is rounded once to 8 bits before it meets the values
 (2^-8 of sum p |v|; FP8: 3 bits for weights under 2^-15 of the row's largest); lse takes no part in
 that rounding; o is rounded once to its own type.
