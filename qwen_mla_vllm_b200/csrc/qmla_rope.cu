@@ -10,8 +10,8 @@
 // block's sines are computed once for all the heads it rotates, and a block walks up to four token groups
 // with the next one's bytes on their way.  Measured on a B200 (copy bandwidth 6.55 TB/s): 32,768 tokens'
 // worth of bf16 pairs side by side 106 us, 3.8 TB/s (one group per block: 128 us); 16,384 tokens into an
-// FP8 cache, queries in place, 117 us, 3.5 TB/s.  What is left is the turning itself: two-byte shared
-// loads and stores of pairs whose halves start at odd offsets, and blocks' phases that do not overlap.
+// FP8 cache, queries in place, 117 us, 3.5 TB/s.  What is left is the turning itself: the update's SMs
+// are 75% busy with two-byte shared loads and stores (halves start at odd offsets), DRAM 38%.
 // Resident warps count most there: eight blocks of 256 threads (32 registers, a few spilled words in the
 // unaligned forms) 117 us, six 156, five 158, two (unbounded registers, four pairs in flight) 209.
 #include <cuda_bf16.h>
