@@ -391,6 +391,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
         for (uint32_t p = count > m.nslots ? count - m.nslots : 0u; p < count; ++p)
           if (p % nlw == lw) mbar_wait(bar(b_full + p % m.nslots), (p / m.nslots) & 1, &never, nullptr, 20000000ull);
       if (lw == 0 && seg > 0) mbar_wait(bar(b_qfull), (seg - 1) & 1, &never, nullptr, 20000000ull);
+      // The peer's copies report to the leader's barriers, which may not even be armed for them when the
+      // leader gave up first: 1 ms, hundreds of times what a copy takes, lets them land.
+      if (cta == 1)
+        for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000000ull;) __nanosleep(2000);
     }
     __syncwarp();
   } else if (warp == kTrMmaWarp) {
@@ -869,6 +873,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves while the other may still signal it or read its tiles
   if (warp == kTrMmaWarp) {
+    // The leader has seen its own arrival of the last commit (b_fin).  The peer's may still be on its way
+    // here, and so may those of the commits before it: this CTA's barriers stay until it is there.
+    volatile int never = 0;
+    if (cta == 1) mbar_wait(bar(b_fin), 0, &never, nullptr, 100000000ull);
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
   }
