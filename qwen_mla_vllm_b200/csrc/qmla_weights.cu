@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
           break;
         }
         tc_fence_after();
-        auto factor = [&](int h) -> float {  // of head h (0 past the last: its column adds 2^-inf)
+        auto factor = [&](int h) -> float {  // of head h (0 past the last)
           if (h >= a.heads) return 0.f;
           if (m.units == 0 || !here) return 1.f;
           const uint8_t* b = tail + m.skip + es * h;
@@ -428,7 +428,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
         const uint32_t ta = tmem + ((uint32_t)(sp * 32) << 16) + grp * m.np;
         float s4[4] = {0.f, 0.f, 0.f, 0.f};
         const bool all_seen = (int64_t)(k + 1) * kTile <= shortest && !cap;
-        // 16 columns at a time; column h * jn + j
+        // 16 columns at a time; column h * jn + j.  A column that adds nothing (no finite lse, or past the
+        // last row) is left out by selection: its score may be NaN, or infinite like its lse.
         auto columns = [&](auto jn_c) {
           constexpr int JN = decltype(jn_c)::value;
           for (int c0 = 0; c0 < m.np; c0 += 16) {
@@ -439,7 +440,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
             for (int i = 0; i < 16; ++i) {
               if (i % JN == 0) f = factor(c0 / JN + i / JN);
               const float2 mt = meta2[c0 + i];
-              s4[i & 3] += ex2_approx(x[i] * f * mt.x * kLog2e - mt.y);
+              const float e = ex2_approx(x[i] * f * mt.x * kLog2e - mt.y);
+              s4[i & 3] += mt.y < INFINITY ? e : 0.f;
             }
           }
         };
@@ -463,7 +465,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
               float s = x[i] * f * mt.x;
               if (cap) s = a.logit_cap * tanhf(s / a.logit_cap);
               const float e = ex2_approx(s * kLog2e - mt.y);
-              if (t < __float_as_int(lim_s[c0 + i])) s4[i & 3] += e;
+              if (t < __float_as_int(lim_s[c0 + i]) && mt.y < INFINITY) s4[i & 3] += e;
               if (++j == m.jn) {
                 j = 0;
                 ++h;
