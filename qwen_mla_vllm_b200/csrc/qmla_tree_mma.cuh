@@ -19,10 +19,15 @@
 // e4m3 form doubles the MMAs at twice the rate), against 224 KB into each SM: up to one group the call
 // is bound by HBM, beyond it by the tensor pipe and the L2-to-SM stream together.
 //
-// Weights P are rounded to bf16; over an FP8 cache to three e5m2 terms (at least 8 bits down to 2^-19 of
-// the row's largest weight, the last of them lost below 2^-29).  Two terms with an e4m3 one among them
-// are a third cheaper in PV but keep 3 bits or none below 2^-15, which a long faint tail behind one heavy
-// token cannot afford.
+// Weights P are rounded to bf16 (8 bits, one operand of the PV instruction, as in the decode kernel);
+// over an FP8 cache to three e5m2 terms (at least 8 bits down to 2^-19 of the row's largest weight, the
+// last of them lost below 2^-29).  The maximum, both sums and O are 32-bit.  O is divided by the sum of the
+// rounded weights, so that the output is a mean of the values with weights off by 2^-9 at most: its error is
+// at most 2^-9 sum_i p_i |v_i - o|, nothing where one token has all the weight; lse comes from the sum of
+// the unrounded ones.  A second bf16 term would cost 24 more MMAs per tile and 16 KB of shared memory,
+// one ring slot of the four that the widest rows leave.  Two terms with an e4m3 one among them are a third
+// cheaper in PV over an FP8 cache but keep 3 bits or none below 2^-15, which a long faint tail behind one
+// heavy token cannot afford.
 // Values of drafted tokens and of the tail of the last page come from a copy with non-finite elements
 // zeroed (prep kernel): a node that does not see such a token has P = 0 there, and 0 * NaN must not
 // reach it; a node that sees it has S = NaN already.
@@ -655,7 +660,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
                                        (a.nodes >= 64 ? ~0ull : (1ull << a.nodes) - 1)
                                  : 0ull;
       const float q_inv = FP8 ? __ldg(m.q_inv + ((int64_t)r * m.groups + g) * 128 + cta * 64 + i) : 1.f;
-      float m_ref = -INFINITY, l_part = 0.f;
+      float m_ref = -INFINITY, l_part = 0.f, l_round = 0.f;  // the sum of P, and of P as PV sees it
       for (int k = k0; k < k1; ++k, ++jt) {
         const uint32_t sb = jt & 1;
         float x[32];
@@ -728,6 +733,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           const float al = mn == m_ref ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - mn);
           m_ref = mn;
           l_part *= al;
+          l_round *= al;
           if (named_bar_or(1, kTrSoft, al != 1.f && k > k0)) {  // (red[] is free again)
             ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
             ok = __all_sync(0xffffffffu, ok);
@@ -749,7 +755,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
         // P = 2^(x - m): nothing where the row sees nothing (m = -inf)
         const float sub = m_ref == -INFINITY && vis != ~0u ? 0.f : m_ref - kShift;
         uint32_t w[FP8 ? 24 : 16];
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        float ls[4] = {0.f, 0.f, 0.f, 0.f}, lr[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (!FP8) {
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -758,11 +764,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
             ls[(e & 2) + 1] += pb;
             const __nv_bfloat162 b = __floats2bfloat162_rn(pa, pb);
             w[e >> 1] = *reinterpret_cast<const uint32_t*>(&b);
+            lr[e & 2] += __uint_as_float(w[e >> 1] << 16);
+            lr[(e & 2) + 1] += __uint_as_float(w[e >> 1] & 0xffff0000u);
           }
         } else {
           // e5m2 is the upper byte of f16: P goes to f16, is rounded there to 9 significant bits, and the
           // three terms are what its upper byte holds, three bits at a time (exact subtractions).
-          // A NaN's bits may wrap in the rounding; it is in l already.
+          // A NaN's bits may wrap in the rounding; it is in l_part already.
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             uint32_t v[2];
@@ -773,6 +781,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
               ls[2 * e + 1] += pb;
               const __half2 hv = __floats2half2_rn(pa, pb);
               v[e] = (*reinterpret_cast<const uint32_t*>(&hv) + 0x00020002u) & 0xfffcfffcu;
+              const float2 pr = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+              lr[2 * e] += pr.x;
+              lr[2 * e + 1] += pr.y;
             }
 #pragma unroll
             for (int t = 0; t < kPTerms; ++t) {
@@ -789,6 +800,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           }
         }
         l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        l_round += (lr[0] + lr[1]) + (lr[2] + lr[3]);
         // the P buffer is free, and O at rest, once the previous tile's PV is done
         if (ok && jt > 0) ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
         ok = __all_sync(0xffffffffu, ok);
@@ -820,7 +832,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       if (dead) break;
       tc_fence_after();
       const float lt = (red[i] + red[64 + i]) + (red[128 + i] + red[192 + i]);
-      const float inv = lt == 0.f ? 0.f : kscale / lt;
+      named_bar_sync(1, kTrSoft);
+      red[quarter * 64 + i] = l_round;
+      named_bar_sync(1, kTrSoft);
+      const float lr = (red[i] + red[64 + i]) + (red[128 + i] + red[192 + i]);
+      const float inv = lt == 0.f ? 0.f : lt != lt ? lt : kscale / lr;
       const bool full = plo >= lo && phi <= hi;
       const int64_t piece = ((int64_t)(plo <= lo ? 2 * range : 2 * range + 1) * m.groups + g) * 128 + cta * 64 + i;
       const int64_t orow = (int64_t)r * a.nodes + node;
