@@ -37,7 +37,8 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
                                         n / b kept, those between blended linearly in turns;
       {"type": "yarn", "factor": f, "original_max_position": n, "beta_fast": 32, "beta_slow": 1,
        "attention_factor": None}        a ramp over the pair index between the pairs that make
-                                        beta_fast and beta_slow turns in n positions; the scale is
+                                        beta_fast and beta_slow turns in n positions (the slow end
+                                        may lie past the last pair, up to rot_dim - 1); the scale is
                                         attention_factor, by default 0.1 ln f + 1.
     """
     if rot_dim < 2 or rot_dim % 2:
@@ -74,7 +75,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
             return rot_dim * math.log(n / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
         lo = max(0.0, math.floor(index(float(scaling.get("beta_fast", 32.0)))))
-        hi = min(half - 1.0, math.ceil(index(float(scaling.get("beta_slow", 1.0)))))
+        hi = min(rot_dim - 1.0, math.ceil(index(float(scaling.get("beta_slow", 1.0)))))
         out = []
         for i, w in enumerate(plain):
             t = min(1.0, max(0.0, (i - lo) / max(hi - lo, 1e-3)))
