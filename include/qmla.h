@@ -333,9 +333,10 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream);
  * rows are tokens ctx_lens[r] .. ctx_lens[r] + num_nodes - 1 of its pages.  Query row
  * r * num_nodes + i is node i of request r; it sees the committed tokens and the drafted tokens j
  * whose bit j is set in tree_mask[r * mask_stride + i] (itself and its ancestors; mask_stride 0:
- * one tree for all requests).  A node whose mask is 0 is padding: o = 0, lse = -inf.  Scores,
- * rms divisors, outputs and strides are qmla_mla_decode's.  A negative length counts as 0; tokens
- * past block_table_cols pages, and pages outside [0, kv_num_pages), count as absent.
+ * one tree for all requests).  A node whose mask is 0 is padding: o = 0, lse = -inf.  Bits at or above
+ * num_nodes name no token; a node with only such bits sees the committed tokens.  Scores, rms
+ * divisors, outputs and strides are qmla_mla_decode's.  A negative length counts as 0; tokens past
+ * block_table_cols pages, and pages outside [0, kv_num_pages), count as absent.
  * What a hidden token's row holds, NaN included, cannot reach a node that does not see it. */
 typedef struct qmla_tree_params {
   const void* q;

@@ -656,9 +656,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     bool ok = true, dead = false;
     while (!dead && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
       const int ctx = tree_ctx(a, r);
-      const uint64_t mask = live ? (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + r * a.mask_stride + node) &
-                                       (a.nodes >= 64 ? ~0ull : (1ull << a.nodes) - 1)
-                                 : 0ull;
+      const uint64_t bits = live ? (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + r * a.mask_stride + node) : 0ull;
+      const bool padding = bits == 0;  // bits past the nodes name no token, but such a node is no padding
+      const uint64_t mask = bits & (a.nodes >= 64 ? ~0ull : (1ull << a.nodes) - 1);
       const float q_inv = FP8 ? __ldg(m.q_inv + ((int64_t)r * m.groups + g) * 128 + cta * 64 + i) : 1.f;
       float m_ref = -INFINITY, l_part = 0.f, l_round = 0.f;  // the sum of P, and of P as PV sees it
       for (int k = k0; k < k1; ++k, ++jt) {
@@ -700,13 +700,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
         }
         // tokens this row sees: committed ones, and drafts of its mask
         const int nc = ctx - (k * kTile + quarter * 32);  // committed tokens from this thread's first on
-        if (nc < 32 || mask == 0) {
+        if (nc < 32 || padding) {
           uint32_t see = nc <= 0 ? 0u : nc >= 32 ? ~0u : (1u << nc) - 1;
           if (nc >= 0)
             see |= nc < 32 ? (uint32_t)(mask << nc) : 0u;
           else
             see |= -nc < 64 ? (uint32_t)(mask >> -nc) : 0u;
-          vis &= mask == 0 ? 0u : see;
+          vis &= padding ? 0u : see;
         }
         float mx = -INFINITY;
         if (vis == ~0u) {
