@@ -752,8 +752,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
             }
           }
         }
-        // P = 2^(x - m): nothing where the row sees nothing (m = -inf)
-        const float sub = m_ref == -INFINITY && vis != ~0u ? 0.f : m_ref - kShift;
+        // P = 2^(x - m): nothing where the row sees nothing, or only scores of -inf, so far (m = -inf)
+        const float sub = m_ref == -INFINITY ? 0.f : m_ref - kShift;
         uint32_t w[FP8 ? 24 : 16];
         float ls[4] = {0.f, 0.f, 0.f, 0.f}, lr[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (!FP8) {
