@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from .mla_decode_attention import _FP8_TYPES, _dt, rms_mode_for
-from .tree_attention import run_with_workspace
+from .tree_attention import run_with_workspace, workspace_bytes
 
 _PACK_WEIGHTS = _lib.packer(_lib.WeightsParams)
 _PACK_EVICT = _lib.packer(_lib.EvictParams)
@@ -29,8 +29,30 @@ def accumulate_attention_weights(q: torch.Tensor, kv_cache: torch.Tensor, weight
     flattened rows (``qrows`` of one request side by side), lse [reqs * qrows, heads] fp32 what it
     returned for them; block_table [reqs, cols] int32.  weights [reqs, columns] fp32: columns at or
     past a request's longest row are left alone.  ``rank`` is needed with a separate ``q_pe`` only
-    (the width of q's latent part).  The row format flags are ``decode_attention_fwd``'s.
+    (the width of q's latent part).  The row format flags are ``decode_attention_fwd``'s; ``workspace`` is
+    as ``tree_attention``'s (``accumulate_attention_weights_workspace_bytes``).
     """
+    args = _weights_args(q, kv_cache, weights, lse, block_table, seq_lens, sm_scale=sm_scale, page_size=page_size,
+                         rank=rank, rms_offset=rms_offset, rms_bf16=rms_bf16, rms_log8=rms_log8, qk_dim=qk_dim,
+                         logit_cap=logit_cap, k_scale=k_scale, q_pe=q_pe, qrows=qrows, decay=decay)
+    if args is not None:
+        run_with_workspace("qmla_accumulate_weights", _PACK_WEIGHTS.pack, args, q.device, workspace)
+
+
+def accumulate_attention_weights_workspace_bytes(q: torch.Tensor, kv_cache: torch.Tensor, weights: torch.Tensor,
+                                                 lse: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                                                 page_size: int, **how) -> int:
+    """Bytes of ``workspace`` that ``accumulate_attention_weights`` of these arguments needs (shapes and
+    types count, not what the tensors hold)."""
+    how.setdefault("sm_scale", 1.0)
+    args = _weights_args(q, kv_cache, weights, lse, block_table, seq_lens, page_size=page_size, **how)
+    return 0 if args is None else workspace_bytes("qmla_accumulate_weights", _PACK_WEIGHTS.pack, args, q.device)
+
+
+def _weights_args(q, kv_cache, weights, lse, block_table, seq_lens, *, sm_scale, page_size, rank=None, rms_offset=-1,
+                  rms_bf16=False, rms_log8=False, qk_dim=None, logit_cap=0.0, k_scale=None, q_pe=None, qrows=1,
+                  decay=1.0) -> tuple | None:
+    """The checked call as qmla_weights_params' fields up to the workspace; None when there is nothing to do."""
     if not all(t.is_cuda for t in (q, kv_cache, weights, lse, block_table, seq_lens)):
         raise ValueError("accumulate_attention_weights: all tensors must be CUDA tensors")
     if any(t is not None and t.device != q.device for t in (kv_cache, weights, lse, block_table, seq_lens, k_scale, q_pe)):
@@ -62,17 +84,17 @@ def accumulate_attention_weights(q: torch.Tensor, kv_cache: torch.Tensor, weight
     if k_scale is not None and k_scale.dtype != torch.float32:
         raise TypeError("k_scale must be an fp32 device scalar")
     if reqs == 0 or heads == 0:
-        return
+        return None
     pe = q_pe if q_pe is not None else q
     mode = rms_mode_for(kv_cache.dtype, rms_offset, rms_bf16, rms_log8)
-    run_with_workspace("qmla_accumulate_weights", _PACK_WEIGHTS.pack, (
+    return (
         q.data_ptr(), q.stride(0), q.stride(1),
         pe.data_ptr() if q_pe is not None else q.data_ptr() + lat * q.element_size(), pe.stride(0), pe.stride(1),
         _dt(q), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), kv_cache.shape[0], width,
         _lib.DT_FP8E4M3 if fp8 else _lib.DT_BF16, page_size, block_table.data_ptr(), block_table.stride(0),
         block_table.shape[1], seq_lens.data_ptr(), reqs, qrows, heads, lat, qk, rms_offset, mode, sm_scale,
         logit_cap or 0.0, decay, k_scale.data_ptr() if k_scale is not None else 0, lse.data_ptr(), lse.stride(0),
-        weights.data_ptr(), weights.stride(0), weights.shape[1]), q.device, workspace)
+        weights.data_ptr(), weights.stride(0), weights.shape[1])
 
 
 def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
@@ -90,7 +112,8 @@ def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
     the new length move into the places given up below it, both in ascending order; the rest stay put.
     Returns new weights and positions [reqs, min(budget, columns)] (0 and -1 past the length) and int32
     lengths, in ``out`` when given; they must not share memory with the inputs.  The requests' pages
-    must not be shared; pages past a new length are free.
+    must not be shared; pages past a new length are free.  ``workspace`` is as ``tree_attention``'s
+    (``evict_cache_workspace_bytes``).
     """
     ts = (kv_cache, weights, positions, block_table, seq_lens)
     if not all(t.is_cuda for t in ts):
@@ -137,3 +160,13 @@ def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
         recent_from.data_ptr() if recent_from is not None else 0, new_w.data_ptr(), new_p.data_ptr(), new_w.stride(0),
         new_w.shape[1], new_l.data_ptr(), reqs), dev, workspace)
     return new_w, new_p, new_l
+
+
+def evict_cache_workspace_bytes(reqs: int, columns: int, budget: int) -> int:
+    """Bytes of ``workspace`` that ``evict_cache`` of ``reqs`` requests and ``columns`` weights each needs."""
+    if reqs < 0 or columns < 0 or budget < 0:
+        raise ValueError(f"{reqs} requests, {columns} columns, budget {budget}: expected no negative number")
+    budget = min(budget, 2**31 - 1)
+    return workspace_bytes("qmla_evict", _PACK_EVICT.pack, (
+        0, 1, 1, 1, 0, 1, 0, 0, 0, 0, 0, 0, 0, columns, 0, 0, budget, 0, 0, 0, 0, 0, min(budget, columns), 0, reqs),
+        torch.device("cuda", 0))

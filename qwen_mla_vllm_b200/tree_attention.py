@@ -19,25 +19,52 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> the curren
 _PACK = _lib.packer(_lib.TreeParams)
 
 
+def _capturing(idx: int) -> bool:
+    """Whether device idx's current stream is being captured into a CUDA graph."""
+    if torch.cuda.current_device() == idx:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(idx):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def device_index(device: torch.device) -> int:
+    return device.index if device.index is not None else torch.cuda.current_device()
+
+
+def workspace_bytes(name: str, pack, args: tuple, device: torch.device) -> int:
+    """Bytes of workspace the call ``qmla_<name>`` with ``args`` asks for."""
+    need = ctypes.c_int64(0)
+    sizer = _SIZER[name]
+    _lib.check(sizer, getattr(_lib.load(), sizer)(pack(*args, 0, 0, device_index(device)), ctypes.byref(need)))
+    return need.value
+
+
 def run_with_workspace(name: str, pack, args: tuple, device: torch.device, workspace: torch.Tensor | None) -> None:
     """Call ``qmla_<name>`` on the current stream with ``args``, its workspace and the device.
 
     Without a ``workspace``, scratch is kept for the stream (calls on two streams never share it) and
-    grown when the library asks for more; it refuses a small one before it launches anything.
+    grown when the library asks for more; it refuses a small one before it launches anything.  A call
+    that is captured into a CUDA graph gets scratch of its own from the graph's memory pool, as torch's
+    own temporaries do: the graph keeps the address, so what is kept for the stream must not be in it.
     """
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+    idx = device_index(device)
     stream = _raw_stream(idx)
     lib = _lib.load()
-    ws = workspace if workspace is not None else _ws.get((idx, stream))
+    if workspace is not None:
+        if workspace.device.type != "cuda" or device_index(workspace.device) != idx or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on cuda:{idx}")
+        ws = workspace
+    elif _capturing(idx):
+        need = workspace_bytes(name, pack, args, device)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    else:
+        ws = _ws.get((idx, stream))
+        if ws is None:
+            ws = _ws[(idx, stream)] = torch.empty(1 << 20, dtype=torch.uint8, device=device)
     ptr, size = (ws.data_ptr(), ws.numel() * ws.element_size()) if ws is not None else (0, 0)
-    p = pack(*args, ptr, size, idx)
-    rc = getattr(lib, name)(p, stream)
+    rc = getattr(lib, name)(pack(*args, ptr, size, idx), stream)
     if rc == _E_WORKSPACE and workspace is None:
-        need = ctypes.c_int64(0)
-        sizer = _SIZER[name]
-        _lib.check(sizer, getattr(lib, sizer)(p, ctypes.byref(need)))
-        ws = torch.empty(max(need.value, 1 << 20), dtype=torch.uint8, device=device)
-        _ws[(idx, stream)] = ws
+        ws = _ws[(idx, stream)] = torch.empty(workspace_bytes(name, pack, args, device), dtype=torch.uint8, device=device)
         rc = getattr(lib, name)(pack(*args, ws.data_ptr(), ws.numel(), idx), stream)
     _lib.check(name, rc)
 
@@ -85,8 +112,30 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse
     tree_mask int64 [reqs, nodes], or [nodes] for one tree shared by all (``tree_masks``); a node
     whose mask is 0 is padding (o = 0, lse = -inf).
     ``qk_dim`` defaults to ``rms_offset``, or the row width without rms; the rms flags are
-    ``decode_attention_fwd``'s.  Scratch is kept per stream, or is ``workspace`` (a uint8 tensor).
+    ``decode_attention_fwd``'s.  Scratch is kept per stream, or is ``workspace``, a contiguous tensor of at
+    least ``tree_attention_workspace_bytes`` bytes, 256-byte aligned.  In a CUDA graph captured with
+    ``torch.cuda.graph`` it comes from the graph's pool; any other capture needs a ``workspace``.
     """
+    args = _tree_args(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, rank=rank, sm_scale=sm_scale,
+                      page_size=page_size, rms_offset=rms_offset, rms_bf16=rms_bf16, rms_log8=rms_log8, qk_dim=qk_dim,
+                      logit_cap=logit_cap, k_scale=k_scale, q_pe=q_pe)
+    if args is not None:
+        run_with_workspace("qmla_tree_attention", _PACK.pack, args, q.device, workspace)
+
+
+def tree_attention_workspace_bytes(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None,
+                                   block_table: torch.Tensor, ctx_lens: torch.Tensor, tree_mask: torch.Tensor, *,
+                                   rank: int, page_size: int, **how) -> int:
+    """Bytes of ``workspace`` that ``tree_attention`` of these arguments needs (shapes and types count, not
+    what the tensors hold)."""
+    how.setdefault("sm_scale", 1.0)
+    args = _tree_args(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, rank=rank, page_size=page_size, **how)
+    return 0 if args is None else workspace_bytes("qmla_tree_attention", _PACK.pack, args, q.device)
+
+
+def _tree_args(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, *, rank, sm_scale, page_size, rms_offset=-1,
+               rms_bf16=False, rms_log8=False, qk_dim=None, logit_cap=0.0, k_scale=None, q_pe=None) -> tuple | None:
+    """The checked call as qmla_tree_params' fields up to the workspace; None when there is nothing to do."""
     if not all(t.is_cuda for t in (q, kv_cache, o, block_table, ctx_lens, tree_mask)):
         raise ValueError("tree_attention: all tensors must be CUDA tensors")
     if any(t is not None and t.device != q.device for t in (kv_cache, o, lse, block_table, ctx_lens, tree_mask, k_scale, q_pe)):
@@ -119,10 +168,10 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse
     if k_scale is not None and k_scale.dtype != torch.float32:
         raise TypeError("k_scale must be an fp32 device scalar")
     if reqs * nodes == 0:
-        return
+        return None
     pe = q_pe if q_pe is not None else q
     mode = rms_mode_for(kv_cache.dtype, rms_offset, rms_bf16, rms_log8)
-    run_with_workspace("qmla_tree_attention", _PACK.pack, (
+    return (
         q.data_ptr(), q.stride(0), q.stride(1),
         pe.data_ptr() if q_pe is not None else q.data_ptr() + rank * q.element_size(), pe.stride(0), pe.stride(1),
         _dt(q), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), kv_cache.shape[0], width,
@@ -131,4 +180,4 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse
         tree_mask.stride(0) if tree_mask.dim() == 2 else 0, reqs, nodes, heads, rank, qk, rms_offset, mode, sm_scale,
         logit_cap or 0.0, k_scale.data_ptr() if k_scale is not None else 0, o.data_ptr(), o.stride(0), o.stride(1), _dt(o),
         lse.data_ptr() if lse is not None else 0, lse.stride(0) if lse is not None else 0,
-        _dt(lse) if lse is not None else _lib.DT_F32), q.device, workspace)
+        _dt(lse) if lse is not None else _lib.DT_F32)
