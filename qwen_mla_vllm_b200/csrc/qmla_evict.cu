@@ -386,12 +386,7 @@ int qmla_evict(const qmla_evict_params* p, void* stream) try {
   const int64_t per_cta = p->cols / C + 1;
   a.keys_fit = per_cta <= kMaxKeys;
   const size_t smem = a.keys_fit ? (size_t)per_cta * 4 : 0;
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    err = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
-  });
-  if (err != cudaSuccess) return QMLA_E_CUDA;
+  if (!allow_smem(evict_select_kernel, kMaxKeys * 4)) return QMLA_E_CUDA;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)p->num_reqs * C);

@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <map>
 #include <mutex>
+#include <utility>
 
 namespace qmla {
 
@@ -28,10 +29,35 @@ inline DevInfo dev_info(int dev) {
   DevInfo d;
   if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
       cudaDeviceGetAttribute(&d.max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) ==
-          cudaSuccess)
+          cudaSuccess) {
     d.ok = true;
-  devs[dev] = d;
+    devs[dev] = d;
+  } else {
+    cudaGetLastError();  // nothing of a failure stays: the next call asks again
+  }
   return d;
+}
+
+// Lets `kernel` have up to `bytes` of dynamic shared memory on the current device.  The limit belongs to
+// the pair of kernel and device: it is set once for each, and a failure is not remembered.
+inline bool allow_smem(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, int> known;
+  int dev;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = known.find({dev, kernel});
+  if (it != known.end() && it->second >= bytes) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();  // the caller's return code says it; it is not the next launch's error
+    return false;
+  }
+  known[{dev, kernel}] = bytes;
+  return true;
+}
+template <typename... A>
+bool allow_smem(void (*kernel)(A...), int bytes) {
+  return allow_smem(reinterpret_cast<const void*>(kernel), bytes);
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

@@ -256,7 +256,9 @@ struct TreePlan {
   int64_t ws_status, ws_prefix, ws_bounds, ws_img, ws_qinv, ws_tail;
 };
 
-// Clusters of the tensor-core kernel that can be resident at once (asked once per device).
+// Clusters of the tensor-core kernel that can be resident at once on `device`, whatever device is current
+// (asked once for each); -1 when the device cannot be asked, which is not remembered.  Lets the kernel have
+// its shared memory there.
 template <bool FP8, int TERMS>
 int resident_clusters(int device) {
   static std::mutex mu;
@@ -264,14 +266,17 @@ int resident_clusters(int device) {
   std::lock_guard<std::mutex> lk(mu);
   auto it = known.find(device);
   if (it != known.end()) return it->second;
+  DeviceGuard dg(device);
+  if (!dg.ok() || !allow_smem(tree_mma_kernel<FP8, TERMS>, kMaxDynSmem)) return -1;
   int n = 0;
-  if (cudaFuncSetAttribute(tree_mma_kernel<FP8, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem) == cudaSuccess) {
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(kTrThreads);
-    cfg.dynamicSmemBytes = kMaxDynSmem;
-    if (cudaOccupancyMaxActiveClusters(&n, tree_mma_kernel<FP8, TERMS>, &cfg) != cudaSuccess) n = 0;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(kTrThreads);
+  cfg.dynamicSmemBytes = kMaxDynSmem;
+  if (cudaOccupancyMaxActiveClusters(&n, tree_mma_kernel<FP8, TERMS>, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // the error is the caller's return code, not the next launch's
+    return -1;
   }
   known[device] = n;
   return n;
@@ -281,39 +286,41 @@ int resident_clusters(int device) {
 // divisors within whole 16-byte units of the row, a query image that leaves room for three K / V
 // slots, and no more groups of 128 query rows than there are clusters.  Everything else is the
 // generic kernel's.
-void plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
+int plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
   pl->mma = false;
   const bool fp8 = p->kv_dtype == QMLA_DT_FP8E4M3;
   const int es = fp8 ? 1 : 2;
   TreeMma& m = pl->m;
   memset(&m, 0, sizeof(m));
-  if (p->rank % 128 != 0 || p->rank > 768 || p->block_table_cols == 0 || p->num_reqs == 0 || p->num_nodes == 0) return;
+  if (p->rank % 128 != 0 || p->rank > 768 || p->block_table_cols == 0 || p->num_reqs == 0 || p->num_nodes == 0)
+    return QMLA_OK;
   m.run = gcd_int(p->page_size, 64);
   m.chunks = (p->qk_dim * es + 127) / 128;
   m.full_chunks = p->qk_dim * es / 128;
   m.v_chunks = p->rank * es / 128;
   m.terms = q_terms(fp8, p->q_dtype);
-  if (m.run < 16 || m.full_chunks < 2) return;
+  if (m.run < 16 || m.full_chunks < 2) return QMLA_OK;
   if (p->rms_mode != QMLA_RMS_NONE) {
     const int bytes = p->num_heads * (!fp8 || p->rms_mode == QMLA_RMS_BF16 ? 2 : 1);
     const int off = p->rms_offset * es;
     m.base_b = off & ~15;
     m.skip = off - m.base_b;
     m.units = (m.skip + bytes + 15) / 16;
-    if (m.units > 7 || m.base_b + 16 * m.units > p->kv_row_width * es) return;
+    if (m.units > 7 || m.base_b + 16 * m.units > p->kv_row_width * es) return QMLA_OK;
   }
   const int64_t rows = (int64_t)p->num_nodes * p->num_heads;
   const int dev = p->device;
   const int clusters = fp8 ? (m.terms == 2 ? resident_clusters<true, 2>(dev) : resident_clusters<true, 3>(dev))
                            : (m.terms == 1 ? resident_clusters<false, 1>(dev) : resident_clusters<false, 2>(dev));
-  if (rows > (int64_t)128 * clusters) return;
+  if (clusters < 0) return QMLA_E_CUDA;
+  if (rows > (int64_t)128 * clusters) return QMLA_OK;
   m.rows = (int)rows;
   m.groups = (int)((rows + 127) / 128);
   m.ranges = std::min(clusters / m.groups, kMaxCtas);
   const int64_t img = (int64_t)m.terms * m.chunks * kTrRows * 128;
   const int64_t fac = (int64_t)p->num_heads * kTrFacPitch * 4;
   const int64_t ring = std::min(di.max_smem, kMaxDynSmem) - 1024 - img - tr_p_bytes(fp8) - fac - 2048;
-  if (ring < 3 * (int64_t)kTrSlot) return;
+  if (ring < 3 * (int64_t)kTrSlot) return QMLA_OK;
   m.nslots = (uint32_t)std::min<int64_t>(kTrMaxSlots, ring / kTrSlot);
   m.img_bytes = (uint32_t)img;
   m.off_q = m.nslots * kTrSlot;
@@ -342,6 +349,7 @@ void plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
   w = align_up(w + (int64_t)2 * m.ranges * m.groups * 128 * 4 * p->rank, 256);
   pl->ws_total = w;
   pl->mma = true;
+  return QMLA_OK;
 }
 
 int make_tree_plan(const qmla_tree_params* p, TreePlan* pl) {
@@ -368,8 +376,8 @@ int make_tree_plan(const qmla_tree_params* p, TreePlan* pl) {
   const int64_t rows = (int64_t)p->num_reqs * p->num_nodes;
   const int64_t blocks = rows * ((p->num_heads + kGenHeads - 1) / kGenHeads);
   if (blocks > INT32_MAX || rows * p->num_heads > INT32_MAX) return QMLA_E_UNSUPPORTED;
-  plan_mma(p, di, pl);
-  if (pl->mma) return QMLA_OK;
+  const int rc = plan_mma(p, di, pl);
+  if (rc != QMLA_OK || pl->mma) return rc;
   // tokens split over blocks until every SM has two
   pl->nsplit = blocks == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(64, 2 * di.sms / blocks));
   int64_t w = 0;
@@ -385,13 +393,7 @@ template <bool FP8>
 int launch_generic(const TreeArgs& a, cudaStream_t st) {
   const int V = FP8 ? 16 : 8;
   const int smem = kGenHeads * ((a.qk_dim + V - 1) / V * V) * 4;
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    err = cudaFuncSetAttribute(tree_generic_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kGenHeads * kMaxRank * 4);
-  });
-  if (err != cudaSuccess) return QMLA_E_CUDA;
+  if (!allow_smem(tree_generic_kernel<FP8>, kGenHeads * kMaxRank * 4)) return QMLA_E_CUDA;
   const int hgroups = (a.heads + kGenHeads - 1) / kGenHeads;
   tree_generic_kernel<FP8><<<dim3(a.reqs * a.nodes * hgroups, a.nsplit), kGenThreads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;

@@ -601,12 +601,7 @@ int launch_mma(const qmla_weights_params* p, const WeightArgs& a, const WeightPl
     const cuuint32_t box[5] = {col, 8, (cuuint32_t)m.cps, (cuuint32_t)(m.run / 8), 1};
     if (!encode_tiled(&maps.wide, FP8, p->kv_cache, 5, dims, strides, box)) return QMLA_E_ALIGNMENT;
   }
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    err = cudaFuncSetAttribute(weights_mma_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem);
-  });
-  if (err != cudaSuccess) return QMLA_E_CUDA;
+  if (!allow_smem(weights_mma_kernel<FP8>, kMaxDynSmem)) return QMLA_E_CUDA;
   for (int j0 = 0; j0 < a.qrows; j0 += pl.jn) {
     m.j0 = j0;
     m.jn = std::min(pl.jn, a.qrows - j0);
