@@ -342,22 +342,20 @@ template <bool FP8, int NB, int NQK, bool PAIR>
 int launch_decode_t(const CacheMaps& maps, const DecodeArgs& a, uint32_t smem,
                     cudaStream_t st) {
   auto k = mla_decode_kernel<FP8, NB, NQK, PAIR>;
+  if (!allow_smem(k, kMaxDynSmem)) return QMLA_E_CUDA;
   static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
   static bool regs_ok = true;
   std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem);
     if constexpr (NQK >= 32) {
       // the warpgroups' setmaxnreg budgets add up to exactly the pool of a CTA launched with
       // kRegsAtLaunch registers per thread; with fewer, a setmaxnreg.inc would wait forever, so
       // such a build is never launched
       cudaFuncAttributes fa;
       // (registers are allocated to a warp in units of 8 per thread)
-      regs_ok = attr_err == cudaSuccess && cudaFuncGetAttributes(&fa, k) == cudaSuccess &&
+      regs_ok = cudaFuncGetAttributes(&fa, k) == cudaSuccess &&
                 (fa.numRegs + 7) / 8 * 8 * kNumThreads >= (int)(kRegsSoftmax + kRegsProducer) * 256;
     }
   });
-  if (attr_err != cudaSuccess) return QMLA_E_CUDA;
   if (!regs_ok) return QMLA_E_UNSUPPORTED;
   k<<<a.G, kNumThreads, smem, st>>>(maps, a);
   return cudaGetLastError() == cudaSuccess ? QMLA_OK : QMLA_E_CUDA;
@@ -902,6 +900,8 @@ int qmla_gather_cache(const qmla_gather_params* p, void* stream) {
                    a.dst_sr % 16 == 0;
   DevInfo di = dev_info(p->device);
   if (!di.ok) return QMLA_E_CUDA;
+  DeviceGuard dg(p->device);
+  if (!dg.ok()) return QMLA_E_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Aligned rows: the staged kernel (whole rows by the bulk-copy engine through a shared-memory
   // ring), as many blocks as are resident at once.
@@ -920,13 +920,7 @@ int qmla_gather_cache(const qmla_gather_params* p, void* stream) {
     bs.stages = std::min(8, std::max(2, atoi(e)));
   if (vec && bs.copy_bytes >= 16 && bulk_smem_bytes(bs) <= 200 * 1024 &&
       getenv("QMLA_GATHER_REGS") == nullptr) {
-    static std::once_flag once;
-    static cudaError_t attr_err = cudaSuccess;
-    std::call_once(once, [] {
-      attr_err = cudaFuncSetAttribute(gather_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kMaxDynSmem);
-    });
-    if (attr_err != cudaSuccess) return QMLA_E_CUDA;
+    if (!allow_smem(gather_bulk_kernel, kMaxDynSmem)) return QMLA_E_CUDA;
     const int smem = bulk_smem_bytes(bs);
     int per_sm = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, gather_bulk_kernel, kBulkThreads, smem) !=

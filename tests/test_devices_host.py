@@ -87,6 +87,31 @@ def calls(dev):
     assert lib.fake_current() == 0 and lib.fake_refused() == 0
 '''
 
+DECODE_CALLS = '''
+def decode(dev, fp8=False):
+    d = cache(dev, fp8)
+    p = packed(_lib.DecodeParams, **d, kv_num_pages=4096, seq_lens=P, num_rows=4, qrows=1, o=P, o_stride_row=24 * 768, o_stride_head=768,
+               lse=P, lse_stride_row=24, lse_dtype=2)
+    return lib.qmla_mla_decode(ctypes.byref(p), None)
+
+
+def gather(dev, fp8=False):
+    p = packed(_lib.GatherParams, src_cache=P, src_stride_page=16 * 1024, src_stride_token=1024, page_size=16, num_pages=64,
+               src_dtype=3 if fp8 else 0, row_elems=1024, rms_offset=1000, rms_heads=24, rms_mode=3, scale=P, block_table=P,
+               block_table_stride=64, block_table_cols=64, cu_seq_lens=P, token_to_seq=P, num_seqs=2, num_tokens=5000, dst=P,
+               dst_stride_row=1024, device=dev)
+    return lib.qmla_gather_cache(ctypes.byref(p), None)
+
+
+for dev in ORDER:
+    for fp8 in (False, True):
+        for f in (decode, gather):
+            before = lib.fake_launches(dev)
+            assert f(dev, fp8=fp8) == 0, (f.__name__, fp8, dev)
+            assert lib.fake_launches(dev) > before
+assert lib.fake_current() == 0 and lib.fake_refused() == 0
+'''
+
 SCRIPTS = {
     "the current device first": "calls(0); calls(1)",
     "another device first": "calls(1); calls(0)",
@@ -121,8 +146,17 @@ def fake_lib(tmp_path_factory):
     return out
 
 
+def check(lib, script):
+    env = dict(os.environ, QMLA_LIB_PATH=str(lib), PYTHONPATH=str(ROOT))
+    r = subprocess.run([sys.executable, "-c", CALLS + script], env=env, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("name", SCRIPTS)
 def test_two_devices(fake_lib, name):
-    env = dict(os.environ, QMLA_LIB_PATH=str(fake_lib), PYTHONPATH=str(ROOT))
-    r = subprocess.run([sys.executable, "-c", CALLS + textwrap.dedent(SCRIPTS[name])], env=env, capture_output=True, text=True, timeout=120)
-    assert r.returncode == 0, r.stderr[-2000:]
+    check(fake_lib, textwrap.dedent(SCRIPTS[name]))
+
+
+@pytest.mark.parametrize("order", ["(0, 1)", "(1, 0)"])
+def test_decode_and_gather_on_two_devices(fake_lib, order):
+    check(fake_lib, f"ORDER = {order}\n" + DECODE_CALLS)
