@@ -409,6 +409,13 @@ typedef struct qmla_weights_params {
 int qmla_weights_workspace_bytes(const qmla_weights_params* p, int64_t* bytes);
 int qmla_accumulate_weights(const qmla_weights_params* p, void* stream);
 
+/* QMLA_STATUS_* bits of the qmla_tree_attention and qmla_accumulate_weights calls on `device` since the
+ * last clear.  Their tensor-core kernels give up a wait that lasts 2 s and set QMLA_STATUS_TIMEOUT, which
+ * does not happen on a sound GPU.  All outputs of such a tree attention are NaN; of such an accumulation
+ * some tokens have their new weight and the others their old one.  Copies eight bytes device->host on
+ * `stream` and synchronises it (not for graph capture); clear != 0 zeroes the bits. */
+int qmla_operator_status(int32_t device, int32_t clear, void* stream, int32_t* status);
+
 /* Keep the K = min(n, budget, budgets[r]) heaviest of request r's n = seq_lens[r] tokens, and
  * close up the cache.  Tokens whose position is below `sinks` or at or past recent_from[r] come
  * before all others, then the larger weight (NaN last), then the lower index.  The i-th kept token at

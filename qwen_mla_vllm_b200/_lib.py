@@ -379,6 +379,7 @@ PROTOTYPES = {
     "qmla_tree_attention": (ctypes.c_int, [_VP, _VP]),
     "qmla_weights_workspace_bytes": (ctypes.c_int, [_VP, ctypes.POINTER(_I64)]),
     "qmla_accumulate_weights": (ctypes.c_int, [_VP, _VP]),
+    "qmla_operator_status": (ctypes.c_int, [_I32, _I32, _VP, ctypes.POINTER(_I32)]),
     "qmla_evict_workspace_bytes": (ctypes.c_int, [_VP, ctypes.POINTER(_I64)]),
     "qmla_evict": (ctypes.c_int, [_VP, _VP]),
     "qmla_rotary": (ctypes.c_int, [_VP, _VP]),

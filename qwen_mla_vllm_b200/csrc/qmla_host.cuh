@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -85,6 +86,25 @@ inline bool encode_tiled(CUtensorMap* m, bool fp8, const void* base, int nd, con
             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+// How long a wait of the tensor-core operators may last.
+inline uint32_t wait_limit_us() {
+  if (const char* e = getenv("QMLA_WAIT_US")) return (uint32_t)atoi(e);  // test hook: 0 gives up at once
+  return 2000000;
+}
+
+// Reads (and clears) a status word in device memory by its symbol, on the current device.
+inline int take_status(const void* symbol, bool clear, cudaStream_t st, int32_t* bits) {
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, symbol) != cudaSuccess ||
+      cudaMemcpyAsync(bits, p, 4, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      (clear && cudaMemsetAsync(p, 0, 4, st) != cudaSuccess) || cudaStreamSynchronize(st) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  return 0;
+}
+int weights_status(bool clear, cudaStream_t st, int32_t* bits);  // the attention weights' word
 
 inline int gcd_int(int a, int b) {
   while (b) {

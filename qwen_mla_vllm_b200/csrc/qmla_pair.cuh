@@ -27,6 +27,34 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Whether a phase is complete, without the suspension that try_wait may bring.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_wait with the launch's own limit; with 0 an unfinished phase is polled until the timer's next step.
+__device__ __forceinline__ bool mbar_wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                              uint32_t limit_us) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (limit_us ? mbar_try_wait_sleep(bar, parity, 20000u) : mbar_test_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > 1000ull * limit_us) {
+      *abort_flag = 1;
+      atomicOr(status, QMLA_DEV_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
 // Tiled loads into this CTA's shared memory whose bytes are counted on an mbarrier of either CTA
 // of the pair (`bar` from map_cta).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, int x, int y, uint32_t bar, uint64_t policy) {

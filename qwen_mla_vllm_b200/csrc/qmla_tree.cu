@@ -404,6 +404,7 @@ int launch_tree_mma(const qmla_tree_params* p, const TreeArgs& a, const TreePlan
   const int es = FP8 ? 1 : 2;
   TreeMma m = pl.m;
   m.status = reinterpret_cast<int*>(ws + pl.ws_status);
+  m.wait_us = wait_limit_us();
   m.prefix = reinterpret_cast<int32_t*>(ws + pl.ws_prefix);
   m.bounds = reinterpret_cast<int32_t*>(ws + pl.ws_bounds);
   m.img = ws + pl.ws_img;
@@ -458,6 +459,19 @@ int qmla_tree_workspace_bytes(const qmla_tree_params* p, int64_t* bytes) try {
   const int rc = make_tree_plan(p, &pl);
   if (rc != QMLA_OK) return rc;
   *bytes = pl.ws_total;
+  return QMLA_OK;
+} catch (...) {  // no exception leaves a C entry
+  return QMLA_E_CUDA;
+}
+
+int qmla_operator_status(int32_t device, int32_t clear, void* stream, int32_t* status) try {
+  if (!status) return QMLA_E_INVALID;
+  DeviceGuard dg(device);
+  if (!dg.ok()) return QMLA_E_CUDA;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int32_t tree = 0, weights = 0;
+  if (take_status(&g_tree_status, clear != 0, st, &tree) != 0 || weights_status(clear != 0, st, &weights) != 0) return QMLA_E_CUDA;
+  *status = tree | weights;
   return QMLA_OK;
 } catch (...) {  // no exception leaves a C entry
   return QMLA_E_CUDA;

@@ -50,6 +50,8 @@
 
 namespace qmla {
 
+__device__ int g_tree_status;  // bits of every call that failed on this device (qmla_operator_status)
+
 struct TreeArgs {
   const uint8_t *q, *q_pe;
   int64_t q_sr, q_sh, qpe_sr, qpe_sh;  // elements
@@ -107,7 +109,8 @@ struct TreeMma {
   uint8_t* tail;     // [reqs][kTrTail][rank]
   float* part_o;     // [2 * ranges][groups][128][rank]
   float* part_lse;   // [2 * ranges][groups][128], log2 units
-  int* status;
+  int* status;               // of this call
+  uint32_t wait_us;          // how long a wait may last
   int groups, ranges, rows;  // rows = nodes * heads
   int terms, chunks, full_chunks, v_chunks;
   int run;                   // tokens per K / V box
@@ -309,13 +312,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       if (lw < nlw) turn = turn + 1 == nlw ? 0u : turn + 1;
     };
     auto slot_begin = [&](uint32_t bytes) {
-      ok = mbar_wait(bar(b_empty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
+      ok = mbar_wait_for(bar(b_empty + ring.idx), ring.ph ^ 1, abort_flag, m.status, m.wait_us);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && cta == 0 && lane == 0) mbar_expect_tx(bar(b_full + ring.idx), bytes);
     };
     while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
       if (lw == 0) {
-        if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
+        if (seg > 0) ok = mbar_wait_for(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status, m.wait_us);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
@@ -410,7 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
     bool ok = true;
     if (cta == 1) {  // tell the leader that this CTA's Q has landed
       while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(b_qfull), seg & 1, abort_flag, m.status));
+        ok = __all_sync(0xffffffffu, mbar_wait_for(bar(b_qfull), seg & 1, abort_flag, m.status, m.wait_us));
         if (ok && lane == 0) mbar_arrive_cluster(leader(b_qpeer));
         ++seg;
       }
@@ -422,7 +425,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       uint32_t js = 0, jp = 0;  // tiles scored / accumulated so far
       Ring ring;
       auto wait = [&](uint32_t b, uint32_t ph) {  // the whole warp
-        ok = ok && mbar_wait(bar(b), ph, abort_flag, m.status);
+        ok = ok && mbar_wait_for(bar(b), ph, abort_flag, m.status, m.wait_us);
         ok = __all_sync(0xffffffffu, ok);
       };
       // The slot at the head of the ring.  Its barrier is tried before the MMAs of the slot before it
@@ -596,7 +599,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           }
         };
         load(0);
-        if (jt > 0) ok = mbar_wait(bar(b_facfree), (jt - 1) & 1, abort_flag, m.status);
+        if (jt > 0) ok = mbar_wait_for(bar(b_facfree), (jt - 1) & 1, abort_flag, m.status, m.wait_us);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
@@ -664,7 +667,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       for (int k = k0; k < k1; ++k, ++jt) {
         const uint32_t sb = jt & 1;
         float x[32];
-        ok = ok && mbar_wait(bar(b_sfull + sb), (jt >> 1) & 1, abort_flag, m.status);
+        ok = ok && mbar_wait_for(bar(b_sfull + sb), (jt >> 1) & 1, abort_flag, m.status, m.wait_us);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           tc_fence_after();
@@ -673,7 +676,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(sempty0 + sb * 8);
-          ok = mbar_wait(bar(b_facfull), jt & 1, abort_flag, m.status);
+          ok = mbar_wait_for(bar(b_facfull), jt & 1, abort_flag, m.status, m.wait_us);
           ok = __all_sync(0xffffffffu, ok);
         }
         uint32_t vis = 0;
@@ -735,7 +738,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
           l_part *= al;
           l_round *= al;
           if (named_bar_or(1, kTrSoft, al != 1.f && k > k0)) {  // (red[] is free again)
-            ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
+            ok = mbar_wait_for(bar(b_odone), (jt - 1) & 1, abort_flag, m.status, m.wait_us);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
               tc_fence_after();
@@ -802,7 +805,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
         l_part += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         l_round += (lr[0] + lr[1]) + (lr[2] + lr[3]);
         // the P buffer is free, and O at rest, once the previous tile's PV is done
-        if (ok && jt > 0) ok = mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
+        if (ok && jt > 0) ok = mbar_wait_for(bar(b_odone), (jt - 1) & 1, abort_flag, m.status, m.wait_us);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           if constexpr (!FP8) {
@@ -826,7 +829,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
       }
       if (dead) break;
       // ---- O / l -> the output, or this range's piece of it
-      ok = ok && mbar_wait(bar(b_odone), (jt - 1) & 1, abort_flag, m.status);
+      ok = ok && mbar_wait_for(bar(b_odone), (jt - 1) & 1, abort_flag, m.status, m.wait_us);
       red[quarter * 64 + i] = l_part;
       dead = named_bar_or(1, kTrSoft, !ok);
       if (dead) break;
@@ -901,9 +904,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTrThreads, 1)
 
 // Joins the pieces of requests cut at range boundaries: o = sum_i 2^(lse_i - lse) o_i.  One block per
 // (request, query row), a thread per four dims, up to eight pieces' loads in flight.  Requests inside
-// one range are final already.
+// one range are final already.  Where a wait of the call gave up nothing is: all its outputs become NaN.
 __global__ void __launch_bounds__(192) tree_pieces_kernel(const TreeArgs a, const TreeMma m) {
   const int r = blockIdx.x, x = blockIdx.y;
+  if (const int failed = *m.status) {
+    const int node = x / a.heads, h = x - node * a.heads;
+    const int64_t row = (int64_t)r * a.nodes + node;
+    for (int e = 0; e < 4; ++e)
+      store_from_float(a.o + (row * a.o_sr + (int64_t)h * a.o_sh + 4 * threadIdx.x + e) * dt_size(a.o_dtype), a.o_dtype, NAN);
+    if (threadIdx.x == 0 && a.lse) store_from_float(a.lse + (row * a.lse_sr + h) * dt_size(a.lse_dtype), a.lse_dtype, NAN);
+    if (threadIdx.x == 0 && r == 0 && x == 0) atomicOr(&g_tree_status, failed);
+    return;
+  }
   __shared__ int bnd[kMaxCtas + 1];
   const int plo = __ldg(m.prefix + r), phi = __ldg(m.prefix + r + 1);
   for (int c = threadIdx.x; c <= m.ranges; c += blockDim.x) bnd[c] = __ldg(m.bounds + c);

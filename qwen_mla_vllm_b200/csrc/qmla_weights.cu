@@ -31,6 +31,8 @@ using namespace qmla;
 
 namespace {
 
+__device__ int g_weights_status;  // bits of every call that failed on this device (qmla_operator_status)
+
 constexpr int kMaxDim = 2048;
 
 struct WeightArgs {
@@ -164,6 +166,7 @@ struct WeightMmaArgs {
   int first;                // this pass applies the decay
   int q_vec;
   int* status;
+  uint32_t wait_us;         // how long a wait may last
 };
 struct WeightMaps {
   CUtensorMap chunk;  // (element, token in page, page), box = one 128-byte column x run tokens
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
     bool ok = true;
     while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
       if (lane == 0) {
-        if (seg > 0) ok = mbar_wait(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status);
+        if (seg > 0) ok = mbar_wait_for(bar(b_qempty), (seg - 1) & 1, abort_flag, m.status, m.wait_us);
         if (ok) {
           mbar_expect_tx(bar(b_qfull), m.img_bytes);
           load_image(qbuf, m.img + (int64_t)r * m.img_bytes, m.img_bytes, bar(b_qfull), policy_evict_last());
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         for (int s = 0; s < m.nslots && ok; ++s) {
           const int c0 = s * m.cps, nch = min(m.cps, m.chunks - c0);
           const bool plain = c0 + m.cps > m.full_chunks;
-          ok = mbar_wait(bar(b_kempty + ring.idx), ring.ph ^ 1, abort_flag, m.status);
+          ok = mbar_wait_for(bar(b_kempty + ring.idx), ring.ph ^ 1, abort_flag, m.status, m.wait_us);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(bar(b_kfull + ring.idx), (uint32_t)nch * 16384u);
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
     Ring ring;
     bool ok = true;
     auto wait = [&](uint32_t b, uint32_t ph) {
-      ok = ok && mbar_wait(bar(b), ph, abort_flag, m.status);
+      ok = ok && mbar_wait_for(bar(b), ph, abort_flag, m.status, m.wait_us);
       ok = __all_sync(0xffffffffu, ok);
     };
     while (ok && next_segment(m.prefix, cur, r, k0, k1, plo, phi)) {
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         }
         float* wp = a.w + r * a.w_sr + t;
         const float old = t < n ? *wp : 0.f;
-        ok = mbar_wait(bar(b_sfull + grp), (jt >> 1) & 1, abort_flag, m.status);
+        ok = mbar_wait_for(bar(b_sfull + grp), (jt >> 1) & 1, abort_flag, m.status, m.wait_us);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -483,6 +486,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_weights_status, QMLA_DEV_ERR_TIMEOUT);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
@@ -582,6 +586,7 @@ int launch_mma(const qmla_weights_params* p, const WeightArgs& a, const WeightPl
   const int es = FP8 ? 1 : 2;
   WeightMmaArgs m = pl.m;
   m.status = reinterpret_cast<int*>(ws + pl.ws_status);
+  m.wait_us = wait_limit_us();
   m.prefix = reinterpret_cast<const int32_t*>(ws + pl.ws_prefix);
   m.meta = reinterpret_cast<const float*>(ws + pl.ws_meta);
   m.img = ws + pl.ws_img;
@@ -615,6 +620,8 @@ int launch_mma(const qmla_weights_params* p, const WeightArgs& a, const WeightPl
 }
 
 }  // namespace
+
+int qmla::weights_status(bool clear, cudaStream_t st, int32_t* bits) { return take_status(&g_weights_status, clear, st, bits); }
 
 extern "C" {
 

@@ -69,6 +69,17 @@ def run_with_workspace(name: str, pack, args: tuple, device: torch.device, works
     _lib.check(name, rc)
 
 
+def operator_status(device: torch.device | int | None = None, clear: bool = True) -> int:
+    """Status bits of the ``tree_attention`` and ``accumulate_attention_weights`` calls on a device since the
+    last clear (1: a wait inside a kernel gave up; such a tree attention returned NaN, such an accumulation
+    left some weights as they were).  Synchronises the current stream."""
+    dev = torch.device("cuda", device) if isinstance(device, int) else (device or torch.device("cuda"))
+    idx = device_index(dev)
+    bits = ctypes.c_int32(0)
+    _lib.check("qmla_operator_status", _lib.load().qmla_operator_status(idx, clear, _raw_stream(idx), ctypes.byref(bits)))
+    return bits.value
+
+
 _E_WORKSPACE = -4
 _SIZER = {"qmla_tree_attention": "qmla_tree_workspace_bytes", "qmla_accumulate_weights": "qmla_weights_workspace_bytes",
           "qmla_evict": "qmla_evict_workspace_bytes"}

@@ -110,5 +110,6 @@ cudaError_t cudaIpcOpenMemHandle(void**, cudaIpcMemHandle_t, unsigned) { return 
 cudaError_t cudaMalloc(void**, size_t) { return cudaErrorNotSupported; }
 cudaError_t cudaMemcpyAsync(void*, const void*, size_t, cudaMemcpyKind, cudaStream_t) { return cudaErrorNotSupported; }
 cudaError_t cudaMemset(void*, int, size_t) { return cudaErrorNotSupported; }
+cudaError_t cudaMemsetAsync(void*, int, size_t, cudaStream_t) { return cudaErrorNotSupported; }
 cudaError_t cudaStreamSynchronize(cudaStream_t) { return cudaSuccess; }
 }
