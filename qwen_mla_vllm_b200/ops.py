@@ -49,7 +49,7 @@ from .cache_eviction import evict_cache as _evict_cache
 from .mla_decode_attention import build_params, run_params
 from .mla_gather import gather_cache_torch
 from .rotary import rope_kv_cache_update as _rope_kv_cache_update
-from .rotary import rotary_embed
+from .rotary import rotate
 from .tree_attention import tree_attention as _tree_attention
 
 
@@ -94,8 +94,7 @@ def _gather_cache_fake(src_cache, dst, block_table, cu_seq_lens, token_to_seq, n
 def rotary(x: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor, start: int, blocks: int,
            interleaved: bool, scale: float, adjoint: bool) -> torch.Tensor:
     """Rotary positions into a new tensor (``qmla_rotary``); differentiable in ``x``."""
-    return rotary_embed(x, positions, steps, start=start, blocks=blocks, interleaved=interleaved, scale=scale,
-                        adjoint=adjoint)
+    return rotate(x, positions, steps, start, blocks, interleaved, scale, adjoint)
 
 
 @rotary.register_fake

@@ -117,7 +117,37 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor, 
     ``interleaved`` pairs dims (2i, 2i + 1), otherwise (i, i + rot_dim / 2) of each block.
     ``adjoint`` applies the transpose: the gradient with respect to x of a loss whose gradient with
     respect to the output is given.  ``out=x`` works in place; None allocates a contiguous output.
+    Differentiable in x; an ``out`` takes no part in autograd and is refused where x needs a gradient.
     """
+    how = (start, blocks, interleaved, scale, adjoint)
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return rotate(x, positions, steps, *how, out)
+    if out is not None:
+        raise RuntimeError("rotary_embed: out= does not support automatic differentiation, but x requires a gradient")
+    return _Rotary.apply(x, positions, steps, *how)
+
+
+class _Rotary(torch.autograd.Function):
+    """The map is linear in x: its gradient is the transposed map of the incoming one, which is the same
+    operator again (and so has a gradient itself)."""
+
+    @staticmethod
+    def forward(ctx, x, positions, steps, *how):
+        ctx.save_for_backward(positions, steps)
+        ctx.how = how
+        return rotate(x, positions, steps, *how)
+
+    @staticmethod
+    def backward(ctx, grad):
+        *how, adjoint = ctx.how
+        grad = grad if grad.stride(-1) == 1 else grad.contiguous()
+        return (rotary_embed(grad, *ctx.saved_tensors, **dict(zip(("start", "blocks", "interleaved", "scale"), how)),
+                             adjoint=not adjoint), *[None] * 7)
+
+
+def rotate(x: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor, start: int, blocks: int, interleaved: bool,
+           scale: float, adjoint: bool, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rotary_embed`` outside of autograd."""
     if not x.is_cuda:
         raise ValueError("rotary_embed: x must be a CUDA tensor")
     if x.dtype not in _DT:
