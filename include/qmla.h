@@ -299,7 +299,7 @@ int qmla_rotary(const qmla_rotary_params* p, void* stream);
  * FP8 cache: x / k_scale rounded once to e4m3 (saturating), rms tail as qmla_fp8_cache_write's
  * (LOG8 or BF16) or NONE.  A negative slot writes no row (padding; its q is rotated all the same).
  * A slot past num_pages * page_size writes none either and ORs QMLA_STATUS_BAD_INDEX into *status
- * (when status is not NULL).  q_out may be q_pe itself. */
+ * (when status is not NULL).  q_out may be q_pe itself.  With num_heads = 0 only rows are written. */
 typedef struct qmla_rope_cache_params {
   const void* q_pe;
   int64_t q_stride_token, q_stride_head;

@@ -565,7 +565,7 @@ int qmla_rotary(const qmla_rotary_params* p, void* stream) try {
 }
 
 int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) try {
-  if (!p || p->num_tokens < 0 || p->num_heads <= 0 || p->rank <= 0 || p->rope_width <= 0 ||
+  if (!p || p->num_tokens < 0 || p->num_heads < 0 || p->rank <= 0 || p->rope_width <= 0 ||
       p->rms_heads < 0 || p->rot_dim < 2 || p->rot_dim % 2 != 0 || p->rope_width % p->rot_dim != 0 ||
       p->page_size <= 0 || p->num_pages < 0)
     return QMLA_E_INVALID;
@@ -582,7 +582,7 @@ int qmla_rope_cache_write(const qmla_rope_cache_params* p, void* stream) try {
     return QMLA_E_INVALID;
   if (p->num_tokens == 0) return QMLA_OK;
   if (p->num_tokens > INT32_MAX) return QMLA_E_UNSUPPORTED;
-  if (!p->q_pe || !p->q_out || !p->latent || !p->k_pe || !p->positions || !p->slot_mapping || !p->steps ||
+  if ((p->num_heads > 0 && (!p->q_pe || !p->q_out)) || !p->latent || !p->k_pe || !p->positions || !p->slot_mapping || !p->steps ||
       !p->kv_cache || (fp8 && !p->k_scale))
     return QMLA_E_INVALID;
   const DevInfo di = dev_info(p->device);

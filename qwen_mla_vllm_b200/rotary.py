@@ -225,7 +225,7 @@ def rope_kv_cache_update(q_pe: torch.Tensor, k_pe: torch.Tensor, kv_c_normed: to
         raise ValueError(f"cache rows of {width} do not hold {rank} + {packed_rope} and the rms of {tail} heads")
     if fp8 and (k_scale is None or k_scale.dtype != torch.float32 or k_scale.device != kv_cache.device):
         raise TypeError("an FP8 cache needs k_scale, an fp32 scalar on the device")
-    if n == 0 or q_pe.shape[1] == 0:
+    if n == 0:
         return q_out
     idx = _index(kv_cache.device)
     p = _PACK_UPDATE.pack(
