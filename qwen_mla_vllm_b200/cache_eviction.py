@@ -97,6 +97,28 @@ def _weights_args(q, kv_cache, weights, lse, block_table, seq_lens, *, sm_scale,
         weights.data_ptr(), weights.stride(0), weights.shape[1])
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two vectors or matrices with dense rows have a byte in common (True where rows of different
+    strides mingle: that is not looked into)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+
+    def rows(t):  # first byte, bytes of a row, bytes between rows, one past the last byte
+        es, many = t.element_size(), t.dim() == 2 and t.shape[0] > 1
+        w, step = t.shape[-1] * es, t.stride(0) * es if many else 0
+        return t.data_ptr(), w, step, t.data_ptr() + (t.shape[0] - 1 if many else 0) * step + w
+
+    pa, wa, sa, ea = rows(a)
+    pb, wb, sb, eb = rows(b)
+    if ea <= pb or eb <= pa:
+        return False
+    step = sa or sb
+    if step == 0 or sa and sb and sa != sb or max(wa, wb) > step:
+        return True
+    apart = (pb - pa) % step  # rows of one grid: they meet in every step or never
+    return apart < wa or apart + wb > step
+
+
 def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
                 seq_lens: torch.Tensor, budget: int, *, page_size: int, sinks: int = 0,
                 recent_from: torch.Tensor | None = None, budgets: torch.Tensor | None = None,
@@ -147,8 +169,9 @@ def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
                 new_l.shape != (reqs,) or new_p.stride() != new_w.stride() or new_w.stride(1) != 1 or new_l.stride(0) != 1 or \
                 any(t.device != dev for t in out):
             raise ValueError(f"out must be fp32 and int32 [{reqs}, >= {keep}] of one layout and int32 [{reqs}]")
-        if {t.untyped_storage().data_ptr() for t in out} & {t.untyped_storage().data_ptr() for t in (weights, positions, seq_lens)}:
-            raise ValueError("out must not share memory with weights, positions or seq_lens")
+        read = [t for t in (weights, positions, seq_lens, block_table, recent_from, budgets) if t is not None]
+        if any(_overlap(a, b) for i, a in enumerate(out) for b in (*read, *out[i + 1:])):
+            raise ValueError("out must not share memory with the inputs, nor its parts with each other")
     if reqs == 0:
         return new_w, new_p, new_l
     es = kv_cache.element_size()
