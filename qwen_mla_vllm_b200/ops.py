@@ -25,14 +25,15 @@ of ``rotary``, ``tree_attention`` and ``cache_eviction``.
     qmla::tree_attention(Tensor q, Tensor kv_cache, Tensor(a!) o, Tensor(b!) lse, Tensor block_table,
                  Tensor ctx_lens, Tensor tree_mask, int rank, float sm_scale, int page_size,
                  int rms_offset, bool rms_bf16, bool rms_log8, float logit_cap, Tensor? k_scale,
-                 Tensor? workspace=None) -> ()
+                 Tensor? workspace=None, Tensor? q_pe=None, int? qk_dim=None) -> ()
     qmla::accumulate_attention_weights(Tensor q, Tensor kv_cache, Tensor(a!) weights, Tensor lse,
                  Tensor block_table, Tensor seq_lens, float sm_scale, int page_size, int rms_offset,
                  bool rms_bf16, bool rms_log8, float logit_cap, Tensor? k_scale, int qrows, float decay,
-                 Tensor? workspace=None) -> ()
+                 Tensor? workspace=None, Tensor? q_pe=None, int? rank=None, int? qk_dim=None) -> ()
     qmla::evict_cache(Tensor(a!) kv_cache, Tensor weights, Tensor positions, Tensor block_table,
                  Tensor seq_lens, Tensor(b!) new_weights, Tensor(c!) new_positions, Tensor(d!) new_lens,
-                 int budget, int page_size, int sinks, Tensor? recent_from, Tensor? workspace=None) -> ()
+                 int budget, int page_size, int sinks, Tensor? recent_from, Tensor? workspace=None,
+                 Tensor? budgets=None) -> ()
 
 ``rms_mode`` of mla_decode is a ``QMLA_RMS_*`` code (0 none, 1 native, 2 bf16 bytes, 3 log8).
 Set ``rms_offset`` < 0 in gather_cache for a 2-byte cache (no rms layout).  ``workspace`` is scratch (the
@@ -141,16 +142,17 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, o: torch.Tensor, lse
                    block_table: torch.Tensor, ctx_lens: torch.Tensor, tree_mask: torch.Tensor, rank: int,
                    sm_scale: float, page_size: int, rms_offset: int, rms_bf16: bool, rms_log8: bool,
                    logit_cap: float, k_scale: Optional[torch.Tensor],
-                   workspace: Optional[torch.Tensor] = None) -> None:
+                   workspace: Optional[torch.Tensor] = None, q_pe: Optional[torch.Tensor] = None,
+                   qk_dim: Optional[int] = None) -> None:
     """Attention of a drafted token tree into ``o`` / ``lse`` (``qmla_tree_attention``)."""
     _tree_attention(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, rank=rank, sm_scale=sm_scale,
                     page_size=page_size, rms_offset=rms_offset, rms_bf16=rms_bf16, rms_log8=rms_log8,
-                    logit_cap=logit_cap, k_scale=k_scale, workspace=workspace)
+                    logit_cap=logit_cap, k_scale=k_scale, workspace=workspace, q_pe=q_pe, qk_dim=qk_dim)
 
 
 @tree_attention.register_fake
 def _tree_attention_fake(q, kv_cache, o, lse, block_table, ctx_lens, tree_mask, rank, sm_scale, page_size, rms_offset,
-                         rms_bf16, rms_log8, logit_cap, k_scale, workspace=None) -> None:
+                         rms_bf16, rms_log8, logit_cap, k_scale, workspace=None, q_pe=None, qk_dim=None) -> None:
     return None
 
 
@@ -159,18 +161,19 @@ def accumulate_attention_weights(q: torch.Tensor, kv_cache: torch.Tensor, weight
                                  block_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float, page_size: int,
                                  rms_offset: int, rms_bf16: bool, rms_log8: bool, logit_cap: float,
                                  k_scale: Optional[torch.Tensor], qrows: int, decay: float,
-                                 workspace: Optional[torch.Tensor] = None) -> None:
+                                 workspace: Optional[torch.Tensor] = None, q_pe: Optional[torch.Tensor] = None,
+                                 rank: Optional[int] = None, qk_dim: Optional[int] = None) -> None:
     """A step's softmax weights added to ``weights`` (``qmla_accumulate_weights``)."""
     _accumulate_attention_weights(q, kv_cache, weights, lse, block_table, seq_lens, sm_scale=sm_scale,
                                   page_size=page_size, rms_offset=rms_offset, rms_bf16=rms_bf16, rms_log8=rms_log8,
                                   logit_cap=logit_cap, k_scale=k_scale, qrows=qrows, decay=decay,
-                                  workspace=workspace)
+                                  workspace=workspace, q_pe=q_pe, rank=rank, qk_dim=qk_dim)
 
 
 @accumulate_attention_weights.register_fake
 def _accumulate_attention_weights_fake(q, kv_cache, weights, lse, block_table, seq_lens, sm_scale, page_size,
                                        rms_offset, rms_bf16, rms_log8, logit_cap, k_scale, qrows, decay,
-                                       workspace=None) -> None:
+                                       workspace=None, q_pe=None, rank=None, qk_dim=None) -> None:
     return None
 
 
@@ -179,13 +182,13 @@ def _accumulate_attention_weights_fake(q, kv_cache, weights, lse, block_table, s
 def evict_cache(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
                 seq_lens: torch.Tensor, new_weights: torch.Tensor, new_positions: torch.Tensor, new_lens: torch.Tensor,
                 budget: int, page_size: int, sinks: int, recent_from: Optional[torch.Tensor],
-                workspace: Optional[torch.Tensor] = None) -> None:
+                workspace: Optional[torch.Tensor] = None, budgets: Optional[torch.Tensor] = None) -> None:
     """Keep each request's heaviest tokens and close up its pages (``qmla_evict``)."""
     _evict_cache(kv_cache, weights, positions, block_table, seq_lens, budget, page_size=page_size, sinks=sinks,
-                 recent_from=recent_from, out=(new_weights, new_positions, new_lens), workspace=workspace)
+                 recent_from=recent_from, out=(new_weights, new_positions, new_lens), workspace=workspace, budgets=budgets)
 
 
 @evict_cache.register_fake
 def _evict_cache_fake(kv_cache, weights, positions, block_table, seq_lens, new_weights, new_positions, new_lens, budget,
-                      page_size, sinks, recent_from, workspace=None) -> None:
+                      page_size, sinks, recent_from, workspace=None, budgets=None) -> None:
     return None
