@@ -9,8 +9,9 @@ kernel); there is no Triton, FlashInfer or CPU path.
 
 ``attn_logits`` stays caller-owned scratch as in the reference: when it is
 large enough it backs the kernel's split workspace, otherwise a per-device
-buffer cached by this module is used (allocated on first use, so make the
-first call outside CUDA-graph capture, as vLLM's warm-up does).
+buffer cached by this module is used.  A call captured with ``torch.cuda.graph``
+takes that scratch from the graph's memory pool instead: a graph keeps the
+address, and the cached buffer is replaced when a call needs a larger one.
 """
 from __future__ import annotations
 
@@ -40,11 +41,21 @@ def _page_stride(buf: torch.Tensor, page_size: int) -> int:
     return buf.stride(-4)
 
 
+def capturing(idx: int) -> bool:
+    """Whether device idx's current stream is being captured into a CUDA graph."""
+    if torch.cuda.current_device() == idx:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(idx):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _workspace(device: torch.device, nbytes: int, scratch: torch.Tensor | None) -> torch.Tensor:
     if scratch is not None and scratch.is_contiguous() and scratch.numel() * scratch.element_size() >= nbytes \
             and scratch.data_ptr() % 256 == 0 and scratch.device == device:
         return scratch
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    if capturing(idx):
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     with _ws_lock:
         ws = _ws_cache.get(idx)
         if ws is None or ws.numel() < nbytes:

@@ -12,19 +12,11 @@ import ctypes
 import torch
 
 from . import _lib
-from .mla_decode_attention import _FP8_TYPES, _dt, rms_mode_for
+from .mla_decode_attention import _FP8_TYPES, _dt, capturing, rms_mode_for
 
 _ws: dict[tuple[int, int], torch.Tensor] = {}
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> the current stream's handle
 _PACK = _lib.packer(_lib.TreeParams)
-
-
-def _capturing(idx: int) -> bool:
-    """Whether device idx's current stream is being captured into a CUDA graph."""
-    if torch.cuda.current_device() == idx:
-        return torch.cuda.is_current_stream_capturing()
-    with torch.cuda.device(idx):
-        return torch.cuda.is_current_stream_capturing()
 
 
 def device_index(device: torch.device) -> int:
@@ -54,7 +46,7 @@ def run_with_workspace(name: str, pack, args: tuple, device: torch.device, works
         if workspace.device.type != "cuda" or device_index(workspace.device) != idx or not workspace.is_contiguous():
             raise ValueError(f"workspace must be a contiguous tensor on cuda:{idx}")
         ws = workspace
-    elif _capturing(idx):
+    elif capturing(idx):
         need = workspace_bytes(name, pack, args, device)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     else:
