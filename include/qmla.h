@@ -422,7 +422,8 @@ int qmla_operator_status(int32_t device, int32_t clear, void* stream, int32_t* s
  * or past K moves, row and all, into the i-th place below K that was given up; every other kept
  * token stays where it is.  new_weights / new_positions [num_reqs][new_cols] get the tokens' weights
  * and positions in their new places, 0 and -1 past K; new_lens gets K.  The outputs must not overlap
- * the inputs, and a request's pages must be its own (not shared with another's prefix). */
+ * the inputs, and a request's pages must be its own (not shared with another's prefix) and lie in the cache: a
+ * row from or to a page outside [0, kv_num_pages) is not moved, its weight and position are. */
 typedef struct qmla_evict_params {
   void* kv_cache; /* any row format: row_bytes are moved */
   int64_t page_stride_bytes, token_stride_bytes, row_bytes, kv_num_pages;

@@ -104,8 +104,9 @@ __device__ __forceinline__ uint64_t cluster_scan(cg::cluster_group& cl, uint64_t
 // cluster's CTAs add up through distributed shared memory; then the tokens equal to it, the
 // movers and the holes are numbered in index order (each warp owns a contiguous run of tokens).
 // A request's keys are read from memory once and stay in shared memory.
-// Bound by its chain of cluster barriers (three passes, two scans), not by bytes: 49 us for 16 requests of
-// up to 65,536 tokens (eight CTAs each), 14 us for 4 of up to 2048.
+// Bound by its chain of passes over the keys (three histograms, two numbered walks), not by bytes: 50 us for 16
+// requests of up to 65,536 tokens (eight CTAs each, a cluster barrier per pass), 15 us for 4 of up to 2048, where a
+// request is one CTA with two keys per thread and no peer to wait for.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ int hists[3][kBins];  // one per pass: none is cleared while the peers may still read it
@@ -252,7 +253,7 @@ constexpr int kMoveRows = 4;  // rows a warp moves together, their loads all in 
 
 // Moves the listed rows, their weights and positions.  A warp takes kMoveRows moves of a request
 // at a time; blocks of a request stride over its list.
-// 89 us for the 16 requests' kept rows past the budget of 12,288 (2 KB rows read and written once).
+// 83 us for the 16 requests' kept rows past the budget of 12,288 (2 KB rows read and written once).
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a) {
   const int r = blockIdx.y, lane = threadIdx.x & 31;
   const int count = __ldg(a.count + r);

@@ -283,8 +283,9 @@ int resident_clusters(int device) {
 }
 
 // The tensor-core kernel takes ranks of whole 128-dim columns up to 768, pages of whole 16-token runs,
-// divisors within whole 16-byte units of the row, a query image that leaves room for three K / V
-// slots, and no more groups of 128 query rows than there are clusters.  Everything else is the
+// divisors within whole 16-byte units of the row, a query image and a factor table (528 bytes per head) that
+// leave room for three K / V slots (not f16 queries of rank 768, nor 48 heads over an FP8 cache of that
+// rank), and no more groups of 128 query rows than there are clusters.  Everything else is the
 // generic kernel's.
 int plan_mma(const qmla_tree_params* p, const DevInfo& di, TreePlan* pl) {
   pl->mma = false;

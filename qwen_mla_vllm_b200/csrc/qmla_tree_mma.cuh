@@ -33,11 +33,13 @@
 // reach it; a node that sees it has S = NaN already.
 //
 // Measured on a B200 (peaks 1663 bf16 TFLOP/s, 6.55 TB/s): 16 requests of up to 32k tokens x 8 nodes x 24
-// heads, rank 768, bf16: 437 us, 208 GF (29% of the peak, the tensor pipe 29% busy, DRAM 17%); 8 x 16 nodes
-// over an FP8 cache 373 us; 16 x 4 nodes x 12 heads, rank 384: 208 us; one request of 517 tokens 37 us.
+// heads, rank 768, bf16: 453 us, 208 GF (28% of the peak, the tensor pipe 29% busy, DRAM 17%); 8 x 16 nodes
+// over an FP8 cache 385 us; 16 x 4 nodes x 12 heads, rank 384: 213 us; one request of 517 tokens 37 us.
 // A 16 x 8 tile takes 10.9k cycles, 4.0k of them QK MMAs and 2.3k PV.  What bounds it is the ring's round
-// trip: beside Q only four 16 KB slots fit, and a slot comes back after about 3000 cycles (empty wait,
-// four boxes, the copy, the MMAs).
+// trip: beside Q only four 16 KB slots fit for its fourteen, and a slot comes back after about 3000 cycles
+// (empty wait, four boxes, the copy, the MMAs).  FP8 has three slots for seven; at rank 384 eight of eight fit and
+// a tile still takes about 8000 cycles: the 48 rows are all CTA 0's, and the softmax and factor work of
+// empty rows is done too.
 //
 // Warps of a CTA: 0-7 softmax and epilogue (a thread owns 32 tokens of one row), 8-10 score factors
 // (1 / rms per token and head), 11 MMA issue (leader) or the announcement that Q has landed (peer), 12-15 TMA loads,
