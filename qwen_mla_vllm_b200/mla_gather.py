@@ -17,6 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .mla_decode_attention import capturing
 
 _DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
 _RMS = {"log8": _lib.RMS_LOG8, "bf16": _lib.RMS_BF16, "e4m3": _lib.RMS_NATIVE}
@@ -34,9 +35,19 @@ def _status_word(device: torch.device) -> torch.Tensor:
     return _status[idx]
 
 
+def status_pointer(device: torch.device) -> int:
+    """Address of the device's status word for a call on the current stream; 0 (no report) for a call inside a
+    capture while there is none yet: made there, its zeroing would run with every replay, and not before."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx not in _status and capturing(idx):
+        return 0
+    return _status_word(device).data_ptr()
+
+
 def gather_status(device: torch.device | int | None = None, clear: bool = True) -> int:
     """Status bits of this device's gathers since the last clear (2 = a row had an index
-    outside the tables and was skipped).  Synchronises the current stream."""
+    outside the tables and was skipped).  Synchronises the current stream.  Calls captured into a graph
+    report here if one outside of a capture came before them on the device."""
     dev = torch.device("cuda", device) if isinstance(device, int) else (device or torch.device("cuda"))
     w = _status_word(dev)
     v = int(w.item())
@@ -112,7 +123,6 @@ def gather_cache_torch(*, src_cache: torch.Tensor, dst: torch.Tensor, block_tabl
     num_seqs = min(bt.shape[0], cu.shape[0] - 1, st.shape[0] if st is not None else bt.shape[0])
     if t2s.shape[0] < num_tokens:
         raise ValueError(f"token_to_seq has {t2s.shape[0]} entries, need {num_tokens}")
-    status = _status_word(dst.device)
     p.src_cache = src_cache.data_ptr()
     p.src_stride_page, p.src_stride_token = src_cache.stride(0), src_cache.stride(1)
     p.page_size, p.num_pages = src_cache.shape[1], src_cache.shape[0]
@@ -121,7 +131,7 @@ def gather_cache_torch(*, src_cache: torch.Tensor, dst: torch.Tensor, block_tabl
     p.seq_starts = st.data_ptr() if st is not None else None
     p.num_seqs, p.num_tokens = max(num_seqs, 0), int(num_tokens)
     p.dst, p.dst_stride_row, p.dst_dtype = dst.data_ptr(), dst.stride(0), _DT[dst.dtype]
-    p.status = status.data_ptr()
+    p.status = status_pointer(dst.device)
     p.device = dst.device.index if dst.device.index is not None else torch.cuda.current_device()
     stream = torch.cuda.current_stream(dst.device).cuda_stream
     _lib.check("qmla_gather_cache", _lib.load().qmla_gather_cache(ctypes.byref(p), ctypes.c_void_p(stream)))

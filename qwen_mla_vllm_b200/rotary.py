@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .mla_gather import _status_word
+from .mla_gather import status_pointer
 from .tree_attention import _raw_stream
 
 _DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
@@ -234,6 +234,6 @@ def rope_kv_cache_update(q_pe: torch.Tensor, k_pe: torch.Tensor, kv_c_normed: to
         slot_mapping.data_ptr(), steps.data_ptr(), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), n,
         kv_cache.shape[0], kv_cache.shape[1], width, _lib.DT_FP8E4M3 if fp8 else _lib.DT_BF16, q_pe.shape[1], rank,
         packed_rope, rot, local_heads, _RMS[rms_mode], interleaved, positions.dtype == torch.int64, scale,
-        k_scale.data_ptr() if fp8 else 0, _status_word(kv_cache.device).data_ptr(), idx)
+        k_scale.data_ptr() if fp8 else 0, status_pointer(kv_cache.device), idx)
     _lib.check("qmla_rope_cache_write", _lib.load().qmla_rope_cache_write(p, _raw_stream(idx)))
     return q_out
